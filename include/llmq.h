@@ -281,6 +281,66 @@ LLMQ_API int llmq_kv_is_integer(const llmq_kv *kv);
 /* Copies an IntAttnKV cache's codes and int32 scales to host buffers. */
 LLMQ_API int llmq_ikv_export(llmq_ctx *ctx, const llmq_kv *kv, int8_t *k, int8_t *v, int32_t *kq, int32_t *vq);
 
+/* ------------------------------------------------ paged KV cache
+ * Keys and values of many sequences in pages of one pool a layer, for
+ * servers whose sequences grow and end at different times; no counterpart in
+ * the reference, whose caches hold one sequence (kvcache.mojo:31-87).  A row
+ * of a page table names a sequence's pages in order: position p is in page
+ * table[seq * width + p / page] at offset p % page.  Pages may be in any
+ * order and shared by sequences (a common prefix).  Tables, lengths and
+ * positions are device memory, read when the kernels run, so a captured
+ * graph follows them.
+ *
+ * Held per position and cached head: LLMQ_PKV_INT8 int8 codes with a float32
+ * scale for the key and for the value, as QuantKV[8] (kvcache.mojo:248-385;
+ * a row with a NaN or an infinity reads back as NaN, one below 2^-120 as
+ * zeros); LLMQ_PKV_F16 float16 values (nearest even, finite values past
+ * 65504 saturate).  page: 64 to 4096 positions, a multiple of 64; head_dim
+ * 64 or 128 (LLMQ_EUNSUPPORTED otherwise). */
+typedef struct llmq_pkv llmq_pkv;
+enum { LLMQ_PKV_INT8 = 0, LLMQ_PKV_F16 = 1 };
+LLMQ_API int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int page, int n_kv, int head_dim,
+                             llmq_pkv **out);
+LLMQ_API int llmq_pkv_free(llmq_pkv *kv);
+LLMQ_API int64_t llmq_pkv_nbytes(const llmq_pkv *kv);
+/* T rows of n_kv heads of keys and values (device floats, rows ld apart)
+ * into `layer`: row t is sequence seq[t]'s position pos[t].  Rows whose
+ * sequence is outside [0, n_seq), whose position is outside the table's row
+ * or whose page is outside the cache are left out (padding: seq or pos -1).
+ * No two rows of a call may name one position. */
+LLMQ_API int llmq_pkv_store(llmq_ctx *ctx, llmq_pkv *kv, int layer, const float *k, const float *v, int64_t ld,
+                            int64_t T, const int32_t *seq, const int32_t *pos, const int32_t *table, int64_t n_seq,
+                            int64_t width);
+/* The rows as the cache holds them, as floats (zeros for rows that store
+ * would leave out). */
+LLMQ_API int llmq_pkv_fetch(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *k, float *v, int64_t ld, int64_t T,
+                            const int32_t *seq, const int32_t *pos, const int32_t *table, int64_t n_seq,
+                            int64_t width);
+/* Attention of one token a sequence: row r's n_head query heads (device
+ * floats, rows ldq apart) over positions 0 .. len[r] - 1 of table row r,
+ * query head h over cached head h / (n_head / n_kv):
+ *   s_j = scale q . k_j;  s_j = cap tanh(s_j / cap) when cap > 0;
+ *   s_j += slopes[h] (j - (len[r] - 1)) when slopes is given;
+ *   out = sum_j softmax(s)_j v_j.
+ * A length of 0 (or less) gives zeros; lengths past the table's row end with
+ * it; positions in pages outside the cache are left out.  work: device
+ * memory of llmq_pkv_work_bytes(kv, rows, n_head) bytes whose contents do
+ * not matter, 16-byte aligned, not shared by calls that may overlap in time.  rows: at most
+ * 65535. */
+LLMQ_API int64_t llmq_pkv_work_bytes(const llmq_pkv *kv, int64_t rows, int n_head);
+LLMQ_API int llmq_pkv_attend(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q,
+                             int64_t ldq, int64_t rows, int n_head, const int32_t *len, const int32_t *table,
+                             int64_t width, float scale, float cap, const float *slopes, void *work,
+                             int64_t work_bytes);
+/* A decode step's attention: row r's new key and value (rows of k and v, ld
+ * apart like q's) are stored at position pos[r] of table row r, then its
+ * query heads attend to positions 0 .. pos[r].  pos[r] < 0: no token, zeros.
+ * No row of a call may attend to a position that another row of it stores. */
+LLMQ_API int llmq_pkv_step(llmq_ctx *ctx, llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q,
+                           const float *k, const float *v, int64_t ld, int64_t rows, int n_head, const int32_t *pos,
+                           const int32_t *table, int64_t width, float scale, float cap, const float *slopes,
+                           void *work, int64_t work_bytes);
+
 /* ------------------------------------------------ GPT-2 (the caller) */
 
 /* load_model (gpt2t.mojo:579-609) from float32 host tensors in Hugging Face

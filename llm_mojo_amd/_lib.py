@@ -21,6 +21,7 @@ class LlmqError(RuntimeError):
 P = ctypes.c_void_p
 I64 = ctypes.c_int64
 I32 = ctypes.c_int
+F32 = ctypes.c_float
 PP = ctypes.POINTER(ctypes.c_void_p)
 
 # name -> (restype, argtypes); the exported C ABI, as declared in include/llmq.h
@@ -67,6 +68,14 @@ SIGNATURES = {
     "llmq_ikv_create": (I32, [P, I32, I32, I32, I32, PP]),
     "llmq_kv_is_integer": (I32, [P]),
     "llmq_ikv_export": (I32, [P, P, P, P, P, P]),
+    "llmq_pkv_create": (I32, [P, I32, I32, I64, I32, I32, I32, PP]),
+    "llmq_pkv_free": (I32, [P]),
+    "llmq_pkv_nbytes": (I64, [P]),
+    "llmq_pkv_store": (I32, [P, P, I32, P, P, I64, I64, P, P, P, I64, I64]),
+    "llmq_pkv_fetch": (I32, [P, P, I32, P, P, I64, I64, P, P, P, I64, I64]),
+    "llmq_pkv_work_bytes": (I64, [P, I64, I32]),
+    "llmq_pkv_attend": (I32, [P, P, I32, P, I64, P, I64, I64, I32, P, P, I64, F32, F32, P, P, I64]),
+    "llmq_pkv_step": (I32, [P, P, I32, P, I64, P, P, P, I64, I64, I32, P, P, I64, F32, F32, P, P, I64]),
     "llmq_gpt2_create": (I32, [P, P, I32, I32, I32, PP]),
     "llmq_gpt2_create_ex": (I32, [P, P, I32, I32, I32, I32, PP]),
     "llmq_gpt2_create_fmt": (I32, [P, P, ctypes.c_char_p, ctypes.c_char_p, I32, PP]),

@@ -96,6 +96,21 @@ int llmq_set_error(int code, const char *fmt, ...);
         if (rc_ != LLMQ_OK) return rc_; \
     } while (0)
 
+// The context's device is the current one while this lives.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const llmq_ctx *ctx) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess)
+            before = now;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard &) = delete;
+    DeviceGuard &operator=(const DeviceGuard &) = delete;
+};
+
 // Runs the enclosing model call on the context's own (non-null) stream, which
 // a decode-step graph can be captured on, after the caller's stream's
 // earlier work; the caller's stream is restored on exit.
