@@ -341,6 +341,45 @@ LLMQ_API int llmq_pkv_step(llmq_ctx *ctx, llmq_pkv *kv, int layer, float *out, i
                            const int32_t *table, int64_t width, float scale, float cap, const float *slopes,
                            void *work, int64_t work_bytes);
 
+/* ------------------------------------------------ rules on logits */
+/* A sampler's rules, in the order they are applied to token v's logit l of a
+ * row; the reference picks from the head's logits as they are
+ * (gpt2t.mojo:792-797).  Each part is device memory or NULL (not applied):
+ *   history: token ids, row r's in history[history_offsets[r] ..
+ *     history_offsets[r + 1] - 1] (rows + 1 offsets); c = how often v is
+ *     there (counted in 32 bits).  Where c > 0: with repetition ([rows]), l = l > 0 ? l /
+ *     repetition[r] : l * repetition[r]; then l -= frequency[r] c +
+ *     presence[r].
+ *   bias_ids, bias, bias_offsets: l += each bias of v in row r's list, in the
+ *     list's order (added to each other first).
+ *   mask: a bit a token, row r's words at mask + r mask_ld, token v bit v %
+ *     32 of word v / 32; a 0 makes l -infinity, whatever it was.
+ * Ids outside the vocabulary are left out, and offsets are taken inside the
+ * lists (history_len and bias_len entries). */
+typedef struct {
+    const int32_t *history;
+    const int64_t *history_offsets;
+    int64_t history_len;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_ids;
+    const float *bias;
+    const int64_t *bias_offsets;
+    int64_t bias_len;
+    const uint32_t *mask;
+    int64_t mask_ld;
+} llmq_logit_rules;
+/* out[rows, V] (rows ldo apart; logits itself, or apart from it) = logits[rows, V] under
+ * the rules (host struct; may be NULL).  pick (device, [rows], or NULL): the
+ * first token of the largest adjusted logit, as the reference's argmax; NaN is
+ * never picked, and a row of nothing but -infinity and NaN gives -1.  work:
+ * with pick, llmq_adjust_logits_work_bytes(rows, V) bytes of device memory
+ * whose contents do not matter, 16-byte aligned, not shared by calls that may
+ * overlap in time.  rows: at most 65535. */
+LLMQ_API int64_t llmq_adjust_logits_work_bytes(int64_t rows, int64_t V);
+LLMQ_API int llmq_adjust_logits(llmq_ctx *ctx, float *out, int64_t ldo, const float *logits, int64_t ldl,
+                                int64_t rows, int64_t V, const llmq_logit_rules *rules, int64_t *pick, void *work,
+                                int64_t work_bytes);
+
 /* ------------------------------------------------ GPT-2 (the caller) */
 
 /* load_model (gpt2t.mojo:579-609) from float32 host tensors in Hugging Face

@@ -76,6 +76,8 @@ SIGNATURES = {
     "llmq_pkv_work_bytes": (I64, [P, I64, I32]),
     "llmq_pkv_attend": (I32, [P, P, I32, P, I64, P, I64, I64, I32, P, P, I64, F32, F32, P, P, I64]),
     "llmq_pkv_step": (I32, [P, P, I32, P, I64, P, P, P, I64, I64, I32, P, P, I64, F32, F32, P, P, I64]),
+    "llmq_adjust_logits_work_bytes": (I64, [I64, I64]),
+    "llmq_adjust_logits": (I32, [P, P, I64, P, I64, I64, I64, P, P, P, I64]),
     "llmq_gpt2_create": (I32, [P, P, I32, I32, I32, PP]),
     "llmq_gpt2_create_ex": (I32, [P, P, I32, I32, I32, I32, PP]),
     "llmq_gpt2_create_fmt": (I32, [P, P, ctypes.c_char_p, ctypes.c_char_p, I32, PP]),
@@ -107,6 +109,13 @@ SIGNATURES = {
     "llmq_llama_generate": (I32, [P, P, I32, I32, I32, P, ctypes.POINTER(ctypes.c_double),
                                   ctypes.POINTER(ctypes.c_double)]),
 }
+
+
+class LogitRules(ctypes.Structure):
+    """llmq_logit_rules (include/llmq.h)."""
+    _fields_ = [("history", P), ("history_offsets", P), ("history_len", I64), ("repetition", P), ("presence", P),
+                ("frequency", P), ("bias_ids", P), ("bias", P), ("bias_offsets", P), ("bias_len", I64), ("mask", P),
+                ("mask_ld", I64)]
 
 
 class LlamaCfg(ctypes.Structure):

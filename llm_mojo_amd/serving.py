@@ -1,6 +1,8 @@
 """What a server calls around the matmuls: the paged key / value cache with
-one token's attention over it (llmq_pkv_*).  No counterpart in the reference,
-whose caches hold one sequence (kvcache.mojo:31-87).
+one token's attention over it (llmq_pkv_*), and a sampler's rules on the
+logits (llmq_adjust_logits).  No counterpart in the reference, whose caches
+hold one sequence (kvcache.mojo:31-87) and whose pick takes the logits as
+they are (gpt2t.mojo:792-797).
 
 Tensors are torch tensors on the context's device; their types and shapes
 are checked here, since the library sees addresses only.
@@ -8,7 +10,7 @@ are checked here, since the library sees addresses only.
 import ctypes
 import math
 
-from ._lib import check, lib
+from ._lib import LogitRules, check, lib
 
 PKV_TYPES = {"int8": 0, "f16": 1}
 
@@ -24,11 +26,11 @@ def _rows(t, heads, hd, name):
 
     _need(t.dtype == torch.float32 and t.is_cuda, f"{name}: a float32 tensor on the GPU")
     if t.dim() == 3:
-        _need(t.shape[1] == heads and t.shape[2] == hd, f"{name}: shape {tuple(t.shape)}, expected {heads} heads of {hd}")
+        _need(t.shape[1] == heads and t.shape[2] == hd, f"{name}: {tuple(t.shape)}, expected {heads} heads of {hd}")
         _need(t.numel() == 0 or (t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd)),
               f"{name}: a row is not in one piece")
     else:
-        _need(t.dim() == 2 and t.shape[1] == heads * hd, f"{name}: shape {tuple(t.shape)}, expected rows of {heads * hd}")
+        _need(t.dim() == 2 and t.shape[1] == heads * hd, f"{name}: {tuple(t.shape)}, expected rows of {heads * hd}")
         _need(t.numel() == 0 or t.stride(1) == 1, f"{name}: a row is not in one piece")
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * hd)
 
@@ -137,3 +139,53 @@ class PagedKV:
             self.free()
         except Exception:
             pass
+
+
+def logits_work_bytes(rows, V):
+    """Bytes of device memory that adjust_logits takes as `work` for a pick."""
+    return lib().llmq_adjust_logits_work_bytes(rows, V)
+
+
+def _vec(t, dtype, n, name):
+    """Address of a contiguous 1-d tensor of n elements (any number for None)."""
+    _need(str(t.dtype) == dtype and t.is_cuda and t.is_contiguous() and t.dim() == 1 and (n is None or t.shape[0] == n),
+          f"{name}: a contiguous {dtype[6:]} tensor{'' if n is None else f' of {n}'} on the GPU")
+    return t.data_ptr()
+
+
+def adjust_logits(ctx, out, logits, history=None, repetition=None, presence=None, frequency=None, bias=None, mask=None,
+                  pick=None, work=None):
+    """out = logits ([rows, V]; out may be logits) under a sampler's rules, in
+    this order: history=(ids, offsets) with repetition, presence and frequency
+    penalties ([rows] each) of its tokens; bias=(ids, values, offsets); mask
+    (int32 [rows, words], a bit a token; 0 forbids it).  pick (int64 [rows]):
+    the first token of the largest result, -1 where none is left."""
+    rows, V = logits.shape
+    for t, name in ((logits, "logits"), (out, "out")):
+        _need(str(t.dtype) == "torch.float32" and t.is_cuda and tuple(t.shape) == (rows, V)
+              and (t.numel() == 0 or t.stride(1) == 1),
+              f"{name}: float32 [{rows}, {V}] on the GPU with rows in one piece")
+    r = LogitRules()
+    if history is not None:
+        r.history, r.history_offsets = (_vec(history[0], "torch.int32", None, "history"),
+                                        _vec(history[1], "torch.int64", rows + 1, "history offsets"))
+        r.history_len = history[0].shape[0]
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if t is not None:
+            setattr(r, name, _vec(t, "torch.float32", rows, name))
+    if bias is not None:
+        n = r.bias_len = bias[0].shape[0]
+        r.bias_ids, r.bias = _vec(bias[0], "torch.int32", n, "bias ids"), _vec(bias[1], "torch.float32", n, "biases")
+        r.bias_offsets = _vec(bias[2], "torch.int64", rows + 1, "bias offsets")
+    if mask is not None:
+        _need(str(mask.dtype) == "torch.int32" and mask.is_cuda and mask.dim() == 2 and mask.shape[0] == rows
+              and (mask.numel() == 0 or mask.stride(1) == 1) and 32 * mask.shape[1] >= V,
+              f"mask: int32 words on the GPU, {rows} rows of {V} bits")
+        r.mask, r.mask_ld = mask.data_ptr(), mask.stride(0) if rows > 1 else max(mask.stride(0), mask.shape[1])
+    w, nw = None, 0
+    if pick is not None:
+        _need(work is not None and work.is_cuda and work.is_contiguous(), "pick: contiguous work memory on the GPU")
+        w, nw = work.data_ptr(), work.numel() * work.element_size()
+    ld = [t.stride(0) if rows > 1 else max(t.stride(0), V) for t in (out, logits)]
+    check(lib().llmq_adjust_logits(ctx.h, out.data_ptr(), ld[0], logits.data_ptr(), ld[1], rows, V, ctypes.byref(r),
+                                   None if pick is None else _vec(pick, "torch.int64", rows, "pick"), w, nw))
