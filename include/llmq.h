@@ -158,7 +158,47 @@ LLMQ_API int llmq_mat_dequant_row(llmq_ctx *ctx, const llmq_mat *mat, int64_t ro
 LLMQ_API int llmq_dot_row_i16(llmq_ctx *ctx, const llmq_mat *mat, int64_t row, int64_t nrows, const int16_t *xq,
                               float *out);
 
+/* Microscaled 4-bit floating point (OCP Microscaling Formats 1.0, MXFP4; no
+ * counterpart in the reference): blocks of 32 along the inputs, each value an
+ * e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 by the low three bits, bit 3 the
+ * sign) times the block's power of two, e8m0 byte e standing for 2^(e - 127)
+ * and 255 for NaN.  Quantizing: e = floor(log2 max|x|) - 2 + 127, at least 0;
+ * codes are the nearest values, ties to the even code, at most 6; a block
+ * with a NaN or an infinity gets e = 255 (its values are all NaN).  Packed,
+ * a row is K / 2 code bytes (column 2 i the low half of byte i) and K / 32
+ * scale bytes; K is a multiple of 32.
+ *
+ * A weight matrix from float32 src[rows, cols] (host, or device with
+ * _device; reduce_rows as in llmq_mat_from_f32), or from packed rows in host
+ * memory (outputs by inputs), which llmq_mat_export_mx4 gives back (either
+ * may be NULL there).  Both operands of its products are microscaled:
+ * llmq_linear, llmq_linear_noalloc and llmq_head quantize their rows of x as
+ * above and then multiply (scratch of llmq_linear_noalloc: T x IN x 17 / 32
+ * bytes and up to 256); under graph capture llmq_linear refuses several
+ * tokens (its workspace is the context's): quantize into memory of your own
+ * and call llmq_mx4_linear. */
+LLMQ_API int llmq_mat_from_f32_mx4(llmq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int reduce_rows,
+                                   llmq_mat **out);
+LLMQ_API int llmq_mat_from_f32_mx4_device(llmq_ctx *ctx, const float *src, int64_t rows, int64_t cols,
+                                          int reduce_rows, llmq_mat **out);
+LLMQ_API int llmq_mat_restore_mx4(llmq_ctx *ctx, int64_t rows, int64_t cols, const uint8_t *codes,
+                                  const uint8_t *scales, llmq_mat **out);
+LLMQ_API int llmq_mat_export_mx4(llmq_ctx *ctx, const llmq_mat *mat, uint8_t *codes, uint8_t *scales);
+
 /* --------------------------------------------------------- compute (device) */
+
+/* T rows of K device floats (ldx apart) to packed codes [T][K / 2] (16-byte
+ * aligned) and scales [T][K / 32], and back to the values they stand for. */
+LLMQ_API int llmq_mx4_quantize(llmq_ctx *ctx, const float *x, int64_t ldx, int64_t T, int64_t K, uint8_t *codes,
+                               uint8_t *scales);
+LLMQ_API int llmq_mx4_dequantize(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scales, int64_t T, int64_t K,
+                                 float *out, int64_t ldo);
+/* linear over rows that llmq_mx4_quantize left (one quantization for several
+ * matrices): out[T, OUT] (+)= act(x @ W^T + bias), w a microscaled matrix;
+ * the same results as llmq_linear on the rows themselves.  Uses no
+ * memory but its arguments.  flags as in llmq_linear. */
+LLMQ_API int llmq_mx4_linear(llmq_ctx *ctx, float *out, const uint8_t *codes, const uint8_t *scales,
+                             const llmq_mat *w, const float *bias, int64_t T, int64_t IN, int64_t OUT, int flags);
 
 /* kernels.quantize_rows (kernels.mojo:400-416): xq[T, K] = round(x / sx),
  * sx[t] = max|x[t]| / 32767 (1 for an all-zero row). */

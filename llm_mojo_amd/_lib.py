@@ -37,6 +37,13 @@ SIGNATURES = {
     "llmq_memcpy_d2h": (I32, [P, P, P, ctypes.c_size_t]),
     "llmq_mat_from_f32": (I32, [P, I32, I32, I32, I32, P, I64, I64, I32, PP]),
     "llmq_mat_from_f32_device": (I32, [P, I32, I32, I32, I32, P, I64, I64, I32, PP]),
+    "llmq_mat_from_f32_mx4": (I32, [P, P, I64, I64, I32, PP]),
+    "llmq_mat_from_f32_mx4_device": (I32, [P, P, I64, I64, I32, PP]),
+    "llmq_mat_restore_mx4": (I32, [P, I64, I64, P, P, PP]),
+    "llmq_mat_export_mx4": (I32, [P, P, P, P]),
+    "llmq_mx4_quantize": (I32, [P, P, I64, I64, I64, P, P]),
+    "llmq_mx4_dequantize": (I32, [P, P, P, I64, I64, P, I64]),
+    "llmq_mx4_linear": (I32, [P, P, P, P, P, P, I64, I64, I64, I32]),
     "llmq_mat_from_gguf": (I32, [P, I32, P, I64, I64, PP]),
     "llmq_mat_free": (I32, [P]),
     "llmq_mat_nbytes": (I64, [P]),

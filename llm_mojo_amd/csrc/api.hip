@@ -87,6 +87,8 @@ int ws_take(llmq_ctx *ctx) {
 
 }  // namespace
 
+bool ctx_capturing(const llmq_ctx *ctx) { return capturing(ctx->stream); }
+
 int ctx_workspace(llmq_ctx *ctx, size_t bytes, void **p, int slot) {
     RC(ws_take(ctx));
     if (bytes > ctx->ws_bytes[slot]) {
@@ -302,6 +304,7 @@ int llmq_mat_free(llmq_mat *m) {
 int64_t llmq_mat_nbytes(const llmq_mat *m) {
     if (!m) return 0;
     if (m->kind == MAT_GGUF) return m->n * m->row_bytes;  // gguf.mojo:507-508
+    if (m->kind == MAT_MX4) return m->n * m->k / 2 + m->n * m->k / 32;
     return m->n * m->k * m->bits / 8 + (m->n * m->k / m->group) * 3;  // tensor.mojo:629-632
 }
 
@@ -448,6 +451,7 @@ int llmq_mat_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *d
         hipFree(d);
         return rc;
     }
+    if (m->kind == MAT_MX4) return mx4_dequant_row(ctx, m, row, dst);
     const int64_t tile = row / LLMQ_TILE_ROWS, r = row % LLMQ_TILE_ROWS;
     std::vector<uint8_t> c(m->CK * 16), z(m->NG);
     std::vector<uint16_t> s(m->NG);
@@ -506,6 +510,7 @@ int llmq_linear(llmq_ctx *ctx, float *out, const float *x, const llmq_mat *w, co
                 int64_t IN, int64_t OUT, int flags) {
     LLMQ_REQUIRE(ctx, "linear: null context");
     RC(check_linear(w, IN, OUT));
+    if (w->kind == MAT_MX4) return launch_mx4_linear(ctx, w, x, T, out, bias, flags);
     if (is_float_act(w)) {
         // matmul_rows (kernels.mojo:285-349) for GGUF and for QuantMatrix
         // with A16 = False: the one-token GEMV (dot_row, tensor.mojo:431-482;
@@ -529,6 +534,8 @@ int llmq_linear_noalloc(llmq_ctx *ctx, float *out, const float *x, const llmq_ma
     LLMQ_REQUIRE(ctx && ctx->scratch, "linear_noalloc: null context");
     RC(check_linear(w, IN, OUT));
     LLMQ_REQUIRE(T >= 1, "linear_noalloc: T must be >= 1");
+    if (w->kind == MAT_MX4)
+        return launch_mx4_linear(ctx, w, x, T, out, bias, flags, ctx->scratch, LLMQ_NOALLOC_SCRATCH_BYTES);
     if (is_float_act(w)) {
         // the one-token GEMV uses no scratch; several tokens of Q4_K keep
         // their fp16 activation record there (the other types use no memory)
@@ -558,7 +565,7 @@ int llmq_ln_linear(llmq_ctx *ctx, float *out, const float *x, const float *ln_w,
                    const float *bias, int64_t T, int64_t IN, int64_t OUT, int flags) {
     LLMQ_REQUIRE(ctx && ln_w && ln_b, "ln_linear: bad arguments");
     RC(check_linear(w, IN, OUT));
-    LLMQ_REQUIRE(w->kind == MAT_QUANT, "ln_linear: GGUF matrices take llmq_layernorm then llmq_linear");
+    LLMQ_REQUIRE(w->kind == MAT_QUANT, "ln_linear: GGUF and microscaled matrices take llmq_layernorm then llmq_linear");
     if (!w->a16) {
         // float activations: one token with the LayerNorm fused into the
         // GEMV; several through the context's workspace, then matmul_rows

@@ -48,8 +48,10 @@ struct llmq_ctx {
 // The context's workspace `slot` of at least `bytes` (api.hip); growing it
 // waits for the context's stream first.  Not for use under graph capture.
 int ctx_workspace(llmq_ctx *ctx, size_t bytes, void **p, int slot = 0);
+// Whether the context's stream is being captured into a graph (api.hip).
+bool ctx_capturing(const llmq_ctx *ctx);
 
-enum { MAT_QUANT = 0, MAT_GGUF = 1 };
+enum { MAT_QUANT = 0, MAT_GGUF = 1, MAT_MX4 = 2 };
 
 struct llmq_mat {
     llmq_ctx *ctx = nullptr;
@@ -410,6 +412,14 @@ int qm_cpg_shift(const llmq_mat *w);
 // LLMQ_GEMM_H16=0 forces the fp32 matrix cores.
 int launch_gguf_gemm(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t ldx, int64_t T, float *out,
                      int64_t ldo, const float *bias, int flags, void *rec = nullptr, int64_t rec_cap = -1);
+// Microscaled matrices (mx4.hip; MAT_MX4: codes and scales in its own
+// layout, CK steps of 128 inputs and NG words of four steps' scales a tile).
+// The product quantizes x[T, w->k] first, into `rec` of rec_cap bytes
+// (mx4_record_bytes), or the context's workspace when rec_cap < 0.
+int64_t mx4_record_bytes(int64_t T, int64_t K);
+int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t T, float *out, const float *bias,
+                      int flags, void *rec = nullptr, int64_t rec_cap = -1);
+int mx4_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *dst);
 // The h16 record (gguf_gemm16.hip): its size for T tokens of K inputs, the
 // record kernel, and the Q4_K matmul over a record.
 int64_t h16_rec_bytes(int64_t T, int64_t K);

@@ -166,6 +166,121 @@ class HipGGUFMatrix:
             pass
 
 
+class HipMX4Matrix:
+    """A microscaled 4-bit floating point matrix on the GPU (e2m1 codes, an
+    e8m0 scale a block of 32 inputs; no reference counterpart).  Its products
+    (linear, head, mx4_linear) quantize their activations the same way."""
+
+    OUT_MAJOR = True
+    FROM_GGUF = False
+    ACT16 = False
+
+    def __init__(self, ctx, handle):
+        self.ctx, self.h = ctx, handle
+        rows, cols = ctypes.c_int64(), ctypes.c_int64()
+        check(lib().llmq_mat_shape(self.h, ctypes.byref(rows), ctypes.byref(cols)))
+        self.rows, self.cols = rows.value, cols.value
+
+    @staticmethod
+    def name():
+        return "mx4"
+
+    @classmethod
+    def from_f32(cls, ctx, src, reduce_rows=True):
+        """src: a float32 [rows, cols] numpy array (host) or torch tensor (device, contiguous)."""
+        h = ctypes.c_void_p()
+        rows, cols = src.shape
+        if isinstance(src, np.ndarray):
+            src = np.ascontiguousarray(src, np.float32)
+            check(lib().llmq_mat_from_f32_mx4(ctx.h, hptr(src), rows, cols, 1 if reduce_rows else 0, ctypes.byref(h)))
+        else:
+            if str(src.dtype) != "torch.float32" or not src.is_cuda or not src.is_contiguous():
+                raise ValueError("from_f32: a contiguous float32 tensor on the GPU")
+            check(lib().llmq_mat_from_f32_mx4_device(ctx.h, dptr(src), rows, cols, 1 if reduce_rows else 0,
+                                                     ctypes.byref(h)))
+        return cls(ctx, h)
+
+    @classmethod
+    def restore(cls, ctx, codes, scales):
+        """From packed rows: codes uint8 [rows, cols / 2], scales uint8 [rows, cols / 32] (numpy)."""
+        codes, scales = np.ascontiguousarray(codes, np.uint8), np.ascontiguousarray(scales, np.uint8)
+        rows, half = codes.shape
+        if scales.shape != (rows, half // 16):
+            raise ValueError("restore: buffer sizes do not match the shape")
+        h = ctypes.c_void_p()
+        check(lib().llmq_mat_restore_mx4(ctx.h, rows, 2 * half, hptr(codes), hptr(scales), ctypes.byref(h)))
+        return cls(ctx, h)
+
+    def export(self):
+        """(codes, scales) as restore takes them."""
+        codes = np.zeros((self.rows, self.cols // 2), np.uint8)
+        scales = np.zeros((self.rows, self.cols // 32), np.uint8)
+        check(lib().llmq_mat_export_mx4(self.ctx.h, self.h, hptr(codes), hptr(scales)))
+        return codes, scales
+
+    def nbytes(self):
+        return lib().llmq_mat_nbytes(self.h)
+
+    def group_size(self):
+        return lib().llmq_mat_group_size(self.h)
+
+    def has_i16(self):
+        return bool(lib().llmq_mat_has_i16(self.h))
+
+    def dequant_row(self, row):
+        dst = np.zeros(self.cols, np.float32)
+        check(lib().llmq_mat_dequant_row(self.ctx.h, self.h, row, hptr(dst)))
+        return dst
+
+    def free(self):
+        if getattr(self, "h", None):
+            lib().llmq_mat_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _mx4_rows(x, codes, scales):
+    """(rows, columns, row stride) of x[T, K] with packed codes[T, K / 2] and scales[T, K / 32]."""
+    T, K = x.shape
+    if str(x.dtype) != "torch.float32" or not x.is_cuda or (x.numel() and x.stride(1) != 1):
+        raise ValueError("mx4: float32 rows in one piece on the GPU")
+    _mx4_packed(codes, scales, T, K)
+    return T, K, x.stride(0) if T > 1 else max(x.stride(0), K)
+
+
+def _mx4_packed(codes, scales, T, K):
+    for t, shape in ((codes, (T, K // 2)), (scales, (T, K // 32))):
+        if str(t.dtype) != "torch.uint8" or not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != shape:
+            raise ValueError(f"mx4: contiguous uint8 codes [{T}, {K // 2}] and scales [{T}, {K // 32}] on the GPU")
+
+
+def mx4_quantize(ctx, x, codes, scales):
+    """Rows x[T, K] to packed e2m1 codes[T, K / 2] and e8m0 scales[T, K / 32] (uint8 tensors)."""
+    T, K, ld = _mx4_rows(x, codes, scales)
+    check(lib().llmq_mx4_quantize(ctx.h, dptr(x), ld, T, K, dptr(codes), dptr(scales)))
+
+
+def mx4_dequantize(ctx, codes, scales, out):
+    """The values that packed rows stand for, into out[T, K]."""
+    T, K, ld = _mx4_rows(out, codes, scales)
+    check(lib().llmq_mx4_dequantize(ctx.h, dptr(codes), dptr(scales), T, K, dptr(out), ld))
+
+
+def mx4_linear(ctx, out, codes, scales, w, bias=None, resid=False, gelu=False):
+    """linear over rows that mx4_quantize left: out (+)= act(x @ w^T + bias)."""
+    _mx4_packed(codes, scales, codes.shape[0], w.cols)
+    if str(out.dtype) != "torch.float32" or not out.is_contiguous() or tuple(out.shape) != (codes.shape[0], w.rows):
+        raise ValueError(f"mx4_linear: a contiguous float32 out[{codes.shape[0]}, {w.rows}]")
+    flags = (LLMQ_BIAS if bias is not None else 0) | (LLMQ_GELU if gelu else 0) | (LLMQ_RESID if resid else 0)
+    check(lib().llmq_mx4_linear(ctx.h, dptr(out), dptr(codes), dptr(scales), w.h, dptr(bias), codes.shape[0], w.cols,
+                                w.rows, flags))
+
+
 def quantize_rows(ctx, x, xq, sx):
     """kernels.quantize_rows (kernels.mojo:400-416) on device tensors."""
     T, K = x.shape
