@@ -166,53 +166,434 @@ struct Attend {
     int n_head;
     float scale, cap;
     const float *slopes;
+    int rows, tiles, shift;
+    int2 *meta;    // [row]: first split, number of splits
+    float2 *ml;    // [split][head]: reference (log2), sum
+    float *sums;   // [split][head][hd]
 };
 
-// One wave a (row, query head), a position at a time, with the running
-// maximum and sum of the softmax; lane = dimension.
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
+
+// Eight int8 codes as float16, exactly: byte u = code + 128 under the
+// exponent byte 0x64 is 1024 + u, less 1152.
+__device__ __forceinline__ h8 halves(uint32_t a, uint32_t b) {
+    union {
+        uint32_t u[4];
+        h2 h[4];
+        h8 v;
+    } r;
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.h[i] = r.h[i] - off;
+    return r.v;
+}
+
+__device__ __forceinline__ h8 as_h8(const uint4 &x) {
+    union {
+        uint4 u;
+        h8 v;
+    } r;
+    r.u = x;
+    return r.v;
+}
+
+// Maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float quarters_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ int64_t row_len(const Layer &c, const Attend &a, int64_t r) {
+    const int64_t n = a.len[r];
+    return pkv::clamp_len(a.k ? n + 1 : n, c.width, c.page);
+}
+
+// Which part of which row workgroup column `slot` takes; every wave finds it
+// by itself from the rows' lengths (a.rows <= kPlanRows).
+struct Part {
+    int row, split, count, first;  // row -1: nothing
+    int64_t blocks;                // blocks a split
+};
+__device__ __forceinline__ Part find_part(const Layer &c, const Attend &a, int B, int slot, int lane) {
+    constexpr int N = pkv::kPlanRows / 64;
+    uint32_t nb[N];
+    int64_t total = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int r = 64 * i + lane;
+        nb[i] = r < a.rows ? (uint32_t)((row_len(c, a, r) + B - 1) / B) : 0;
+        total += nb[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    Part p;
+    p.blocks = pkv::split_blocks(total, a.shift);
+    p.row = -1;
+    uint32_t before = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (64 * i >= a.rows) break;
+        const uint32_t mine = 64 * i + lane < a.rows ? pkv::row_splits(nb[i], (uint32_t)p.blocks) : 0;
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(incl, o);
+            if (lane >= o) incl += up;
+        }
+        const uint32_t all = __shfl(incl, 63);
+        if (p.row < 0 && (uint32_t)slot < before + all) {
+            const int at = __popcll(__ballot(before + incl <= (uint32_t)slot));  // < 64
+            const uint32_t end = __shfl(incl, at), n = __shfl(mine, at);
+            p.row = 64 * i + at;
+            p.count = (int)n;
+            p.first = (int)(before + end - n);
+            p.split = slot - p.first;
+        }
+        before += all;
+    }
+    return p;
+}
+
+// Attention of one token over a row's pages, or a split of it: 4 waves, up to
+// 8 query heads of one cached head, on the fp16 matrix cores.
+//
+// Scores: K (16 positions x 32 dimensions) times the queries as 16 columns,
+// columns 0-7 their float16 roundings and 8-15 what those leave times 2^11
+// (22 bits in all; the keys are exact), so column n and n ^ 8 add up to a
+// score, in lane n for positions 4 (lane / 16) + 0..3 of the tile.  Values:
+// the weights are already where the second product wants its rows: row n
+// holds head n's weights as float16, row n ^ 8 what is left times 2^11, and
+// the slots of paged_plan.h give the values in the same order, so nothing is
+// moved between lanes.  For int8 a weight is p times the value's scale over a
+// power of two near the largest scale so far.
+//
+// The reference of a head's exponentials is moved (and the sums rescaled)
+// only when a score passes it by 2^6, which is rare after the first blocks.
+// Each wave keeps its own and reads every fourth block; the four are put
+// together through LDS.  A wave's next keys are on their way while it forms
+// the weights, its next values while it scores.
 template <int HD, int ELEM>
-__global__ __launch_bounds__(64) void pkv_attend_kernel(Layer c, Attend a) {
-    const int64_t r = blockIdx.y;
-    const int h = blockIdx.x, kvh = h / (a.n_head / c.n_kv), lane = threadIdx.x;
-    const int32_t *row = c.table + r * c.width;
-    int64_t len = a.len[r];
-    if (a.k) {
-        const int64_t p = len;
-        len = p < 0 ? 0 : p + 1;
-        const int page = pkv::page_of(row, c.width, c.page, c.pages, p);
-        // every query head of the group writes the same bytes, which its own wave reads below
+__global__ __launch_bounds__(256, 2) void pkv_attend_kernel(Layer c, Attend a) {
+    constexpr int B = ELEM == 1 ? 64 : 32, NT = B / 16, NC = HD * ELEM / 64, NF = HD / 32, ND = HD / 16;
+    constexpr int kBlock = HD * 64;  // bytes of a block's keys, and of its values
+    __shared__ __align__(16) _Float16 qp[16][HD];
+    __shared__ float qexp[8];
+    __shared__ float2 wml[pkv::kWaves][8];
+    __shared__ float wsum[pkv::kWaves][8][HD];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, q = lane >> 4;
+    const int kvh = blockIdx.y / a.tiles, G = a.n_head / c.n_kv, t0 = blockIdx.y % a.tiles * 8;
+    const int h0 = kvh * G + t0, hn = min(8, G - t0);
+
+    Part part;
+    if (a.shift >= 0) {
+        part = find_part(c, a, B, blockIdx.x, lane);
+        if (part.row < 0) return;  // the same for the whole workgroup
+    } else {
+        part = Part{(int)blockIdx.x, 0, 1, 0, 0x7fffffff};
+    }
+    const int64_t r = __builtin_amdgcn_readfirstlane(part.row);
+    const int32_t *table = c.table + r * c.width;
+    const int64_t len = row_len(c, a, r);
+    const int nb = (int)((len + B - 1) / B);
+    const int64_t e64 = (part.split + 1) * part.blocks;
+    const int b0 = __builtin_amdgcn_readfirstlane((int)(part.split * part.blocks)),
+              b1 = __builtin_amdgcn_readfirstlane((int)(e64 < nb ? e64 : nb));
+    const int count = __builtin_amdgcn_readfirstlane(part.count);
+
+    // the new token's rows, by the workgroups whose split ends with it (the
+    // tiles of a group write the same bytes, and each reads its own)
+    if (a.k && len > 0 && b1 == nb && w == pkv::kWaves - 1) {
+        const int64_t p = len - 1;
+        const int page = a.len[r] == p ? pkv::page_of(table, c.width, c.page, c.pages, p) : -1;
         if (page >= 0)
             store_row<HD, ELEM>(c, page, (int)(p % c.page), kvh, a.k + r * a.ldq + kvh * HD, a.v + r * a.ldq + kvh * HD,
                                 lane);
-        __threadfence_block();
     }
-    len = pkv::clamp_len(len, c.width, c.page);
-    float q[HD / 64], o[HD / 64], m = -INFINITY, l = 0.0f;
+    // queries to their planes: heads 2 w and 2 w + 1
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        q[i] = a.q[r * a.ldq + h * HD + lane + 64 * i];
-        o[i] = 0.0f;
+    for (int i = 0; i < 2; i++) {
+        const int h = 2 * w + i;
+        float x[HD / 64], m = 0.0f;
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) {
+            x[d] = h < hn ? a.q[r * a.ldq + (int64_t)(h0 + h) * HD + lane + 64 * d] : 0.0f;
+            m = fmaxf(m, fabsf(x[d]));
+        }
+        m = llmq_wave_max_all(m);
+        const int e = m > 0.0f ? (int)(__float_as_uint(m) >> 23) - 127 : 0;
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) {
+            const float y = ldexpf(x[d], -e);
+            const _Float16 hi = (_Float16)y;
+            qp[h][lane + 64 * d] = hi;
+            qp[h + 8][lane + 64 * d] = (_Float16)((y - (float)hi) * 2048.0f);
+        }
+        if (lane == 0) qexp[h] = ldexpf(a.scale, e);
     }
-    const float slope = a.slopes ? a.slopes[h] : 0.0f;
-    for (int64_t j = 0; j < len; j++) {
-        const int page = pkv::page_of(row, c.width, c.page, c.pages, j);
-        if (page < 0) continue;
-        float k[HD / 64], v[HD / 64], s = 0.0f;
-        load_row<HD, ELEM>(c, page, (int)(j % c.page), kvh, k, v, lane);
+    __syncthreads();
+    h8 qf[NF];
 #pragma unroll
-        for (int i = 0; i < HD / 64; i++) s = fmaf(q[i], k[i], s);
-        s = llmq_wave_sum_all(s) * a.scale;
-        if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
-        s += slope * (float)(j - (len - 1));
-        const float mn = fmaxf(m, s), old = m == mn ? 1.0f : expf(m - mn), e = expf(s - mn);
-        m = mn;
-        l = l * old + e;
-#pragma unroll
-        for (int i = 0; i < HD / 64; i++) o[i] = fmaf(e, v[i], o[i] * old);
+    for (int f = 0; f < NF; f++) {
+        const int d = ELEM == 1 ? (f >> 1) * 64 + q * 16 + (f & 1) * 8 : f * 32 + q * 8;
+        qf[f] = *reinterpret_cast<const h8 *>(&qp[n][d]);
     }
+    const bool low = n >= 8;
+    const float mul = qexp[n & 7];
+    const float own = low ? 0x1p-11f : 1.0f, oth = low ? 1.0f : 0x1p-11f;  // a score from the two columns
+    const float wg = low ? 2048.0f : 1.0f, wr = low ? -2048.0f : 0.0f;     // a weight to its row's share
+    const float slope = a.slopes && (n & 7) < hn ? a.slopes[h0 + (n & 7)] : 0.0f;
+    const bool bias = a.slopes != nullptr;
+
+    const int bpp = c.page / B;
+    const int64_t head_bytes = (int64_t)c.page * HD * ELEM;
+    const uint32_t koff = (uint32_t)(n * HD * ELEM + q * 16), voff = (uint32_t)(n * 64 + q * 16);
+    struct Where {
+        const uint8_t *k, *v;
+        const float *ks, *vs;
+        int live;
+    };
+    auto where = [&](int b) {
+        Where x;
+        const int p = __builtin_amdgcn_readfirstlane(b / bpp), o = b - p * bpp;
+        const int page = __builtin_amdgcn_readfirstlane(table[p]);
+        const bool ok = page >= 0 && page < c.pages;
+        const int64_t hr = (int64_t)(ok ? page : 0) * c.n_kv + kvh;
+        x.k = c.k + hr * head_bytes + (int64_t)o * kBlock;
+        x.v = c.v + hr * head_bytes + (int64_t)o * kBlock;
+        x.ks = ELEM == 1 ? c.ks + hr * c.page + o * B : nullptr;
+        x.vs = ELEM == 1 ? c.vs + hr * c.page + o * B : nullptr;
+        const int64_t left = len - (int64_t)b * B;
+        x.live = ok ? (int)(left < B ? left : B) : 0;
+        return x;
+    };
+    uint4 kr[NT * NC], vr[ND];
+    float4 ks[NT], vs[NT];
+    auto load_k = [&](const Where &x) {
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++)
-        a.out[r * a.ldo + h * HD + lane + 64 * i] = l == 0.0f ? 0.0f : o[i] / l;
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+                kr[t * NC + i] = *reinterpret_cast<const uint4 *>(x.k + koff + t * 16 * HD * ELEM + i * 64);
+            if constexpr (ELEM == 1) {
+                ks[t] = *reinterpret_cast<const float4 *>(x.ks + 16 * t + 4 * q);
+                vs[t] = *reinterpret_cast<const float4 *>(x.vs + 16 * t + 4 * q);
+            }
+        }
+    };
+    auto load_v = [&](const Where &x) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) vr[d] = *reinterpret_cast<const uint4 *>(x.v + voff + d * 1024);
+    };
+
+    v4f acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = kLowest, ref2 = kLowest, l = 0.0f;  // ref2 = ref log2 e, rounded once
+    int ve = ELEM == 1 ? -100 : 0;                   // the weights' power of two
+
+    int b = b0 + w;
+    Where cur{};
+    if (b < b1) {
+        cur = where(b);
+        load_k(cur);
+        load_v(cur);
+    }
+    for (; b < b1; b += pkv::kWaves) {
+        const int live = cur.live, j0 = b * B;
+        const bool more = b + pkv::kWaves < b1;
+        Where next{};
+        if (more) next = where(b + pkv::kWaves);
+        // scores
+        v4f s[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const uint4 x = kr[t * NC + i];
+                if constexpr (ELEM == 1) {
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x.x, x.y), qf[2 * i], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x.z, x.w), qf[2 * i + 1], s[t], 0, 0, 0);
+                } else {
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(x), qf[i], s[t], 0, 0, 0);
+                }
+            }
+        }
+        float sv[NT * 4], vsc[NT * 4];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = s[t][i] * own + llmq_dppf<0x128>(s[t][i]) * oth;  // row_ror:8
+                if constexpr (ELEM == 1) {
+                    x *= reinterpret_cast<const float *>(&ks[t])[i];
+                    vsc[4 * t + i] = reinterpret_cast<const float *>(&vs[t])[i];
+                }
+                sv[4 * t + i] = x * mul;
+            }
+        if (more) load_k(next);
+        if (a.cap > 0.0f)
+#pragma unroll
+            for (int i = 0; i < NT * 4; i++) sv[i] = a.cap * ref_tanhf(sv[i] / a.cap);
+        if (bias) {
+            const float base = (float)(j0 + 4 * q - (len - 1));
+#pragma unroll
+            for (int i = 0; i < NT * 4; i++) sv[i] = fmaf(slope, base + (float)(16 * (i >> 2) + (i & 3)), sv[i]);
+        }
+        if (live < B) {  // the row's end, or a page that is none
+#pragma unroll
+            for (int i = 0; i < NT * 4; i++) {
+                const bool in = 16 * (i >> 2) + 4 * q + (i & 3) < live;
+                sv[i] = in ? sv[i] : -INFINITY;
+                if constexpr (ELEM == 1) vsc[i] = in ? vsc[i] : 0.0f;
+            }
+            if constexpr (ELEM == 2) {  // what lies there may be NaN
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    uint32_t *u = reinterpret_cast<uint32_t *>(&vr[d]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int p = 16 * (i >> 1) + 4 * q + 2 * (i & 1);
+                        u[i] &= p + 1 < live ? 0xffffffffu : (p < live ? 0xffffu : 0u);
+                    }
+                }
+            }
+        }
+        float mx = sv[0], vm = 0.0f;
+#pragma unroll
+        for (int i = 1; i < NT * 4; i++) mx = fmaxf(mx, sv[i]);
+        mx = quarters_max(mx);
+        int nve = ve;
+        if constexpr (ELEM == 1) {
+#pragma unroll
+            for (int i = 0; i < NT * 4; i++) vm = fmaxf(vm, vsc[i]);
+            vm = quarters_max(vm);
+            nve = max(ve, (int)(__float_as_uint(vm) >> 23) - 127);
+        }
+        if (__any(mx > ref + 4.0f || nve > ve)) {  // 4 log2 e < 6
+            const float to = fmaxf(ref, mx), to2 = to * kLog2e;
+            const float f = ref == to ? 1.0f : exp2f(ref2 - to2), fl = ldexpf(f, ve - nve);
+            ref = to;
+            ref2 = ref == kLowest ? kLowest : to2;
+            ve = nve;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = __shfl(fl, 4 * q + i);  // of row 4 q + i
+#pragma unroll
+                for (int d = 0; d < ND; d++) acc[d][i] *= x;
+            }
+        }
+        const float unit = ldexpf(1.0f, 8 - ve);
+        h8 wf[NT / 2];
+#pragma unroll
+        for (int i = 0; i < NT * 4; i++) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sv[i], kLog2e, -ref2));
+            l += p;
+            const float x = ELEM == 1 ? p * (vsc[i] * unit) : p * unit;
+            const float hi = (float)(_Float16)x;
+            // row n: x rounded; row n ^ 8: what that leaves times 2^11 (exact)
+            wf[i >> 3][i & 7] = (_Float16)fmaf(hi, wr, x * wg);
+        }
+        // values
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const uint4 x = vr[d];
+            if constexpr (ELEM == 1) {
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[0], halves(x.x, x.y), acc[d], 0, 0, 0);
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[1], halves(x.z, x.w), acc[d], 0, 0, 0);
+            } else {
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[0], as_h8(x), acc[d], 0, 0, 0);
+            }
+        }
+        if (more) {
+            load_v(next);
+            cur = next;
+        }
+    }
+    // the four waves' results
+    l = quarters_sum(l);
+    if (lane < 8) wml[w][n] = make_float2(ref2, l);
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = acc[d][i], y = __shfl_xor(x, 32);  // rows 4 q + i and 4 q + i + 8
+            if (q < 2) wsum[w][4 * q + i][16 * d + n] = ldexpf(fmaf(y, 0x1p-11f, x), ve - 8);
+        }
+    __syncthreads();
+    if (tid == 0 && blockIdx.y == 0 && part.split == 0 && a.shift >= 0) a.meta[r] = make_int2(part.first, count);
+    for (int i = tid; i < hn * HD; i += 256) {
+        const int h = i / HD, d = i % HD;
+        float R = kLowest, L = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int k = 0; k < pkv::kWaves; k++) R = fmaxf(R, wml[k][h].x);
+#pragma unroll
+        for (int k = 0; k < pkv::kWaves; k++) {
+            const float f = exp2f(wml[k][h].x - R);
+            L = fmaf(wml[k][h].y, f, L);
+            o = fmaf(wsum[k][h][d], f, o);
+        }
+        if (count == 1) {
+            a.out[r * a.ldo + (int64_t)(h0 + h) * HD + d] = L == 0.0f ? 0.0f : o / L;
+        } else {
+            const int64_t at = (int64_t)blockIdx.x * a.n_head + h0 + h;
+            a.sums[at * HD + d] = o;
+            if (d == 0) a.ml[at] = make_float2(R, L);
+        }
+    }
+}
+
+// The splits of a row put together, in their order: a workgroup a (head, row).
+template <int HD>
+__global__ __launch_bounds__(256) void pkv_join_kernel(Attend a) {
+    __shared__ float wl[pkv::kWaves], ws[pkv::kWaves][HD];
+    const int64_t r = blockIdx.y;
+    const int h = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int2 m = a.meta[r];
+    if (m.y <= 1) return;
+    const float2 *ml = a.ml + (int64_t)m.x * a.n_head + h;
+    const float *sums = a.sums + ((int64_t)m.x * a.n_head + h) * HD;
+    float R = kLowest;
+    for (int i = lane; i < m.y; i += 64) R = fmaxf(R, ml[(int64_t)i * a.n_head].x);
+    R = llmq_wave_max_all(R);
+    float L = 0.0f, o[HD / 64] = {};
+#pragma unroll 4
+    for (int i = w; i < m.y; i += pkv::kWaves) {
+        const float2 x = ml[(int64_t)i * a.n_head];
+        const float f = exp2f(x.x - R);
+        L = fmaf(x.y, f, L);
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) o[d] = fmaf(sums[(int64_t)i * a.n_head * HD + lane + 64 * d], f, o[d]);
+    }
+    if (lane == 0) wl[w] = L;
+#pragma unroll
+    for (int d = 0; d < HD / 64; d++) ws[w][lane + 64 * d] = o[d];
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        const int d = threadIdx.x;
+        const float all = (wl[0] + wl[1]) + (wl[2] + wl[3]), s = (ws[0][d] + ws[1][d]) + (ws[2][d] + ws[3][d]);
+        a.out[r * a.ldo + (int64_t)h * HD + d] = all == 0.0f ? 0.0f : s / all;
+    }
 }
 
 template <class F>
@@ -260,7 +641,7 @@ int check_rows(const char *name, const llmq_pkv *kv, const void *k, const void *
     return LLMQ_OK;
 }
 
-int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, const Attend &a, int64_t rows,
+int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, Attend a, int64_t rows,
            const int32_t *table, int64_t width, void *work, int64_t work_bytes) {
     RC(check_cache(name, ctx, kv, layer, table, width, rows));
     LLMQ_REQUIRE((a.out && a.q && a.len && work) || rows == 0, "%s: null argument", name);
@@ -275,11 +656,28 @@ int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, const
     LLMQ_REQUIRE(work_bytes >= want, "%s: %lld bytes of work, %lld needed", name, (long long)work_bytes,
                  (long long)want);
     if (rows == 0) return LLMQ_OK;
+    LLMQ_REQUIRE((uintptr_t)work % 16 == 0, "%s: work is 16-byte aligned", name);
     DeviceGuard guard(ctx);
     const Layer c = layer_of(kv, layer, table, width);
+    const pkv::Plan p = pkv::plan_of(rows, a.n_head, kv->n_kv);
+    const pkv::Work at = pkv::work_of(p, rows, a.n_head, kv->hd);
+    LLMQ_REQUIRE((int64_t)kv->n_kv * p.tiles <= 65535, "%s: %d query heads", name, a.n_head);
+    a.rows = (int)rows;
+    a.tiles = p.tiles;
+    a.shift = p.shift;
+    a.meta = static_cast<int2 *>(work);
+    a.ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(work) + at.ml);
+    a.sums = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + at.sums);
+    // tables too short for a second split need no joining
+    const bool join = p.shift >= 0 && width * kv->page > (int64_t)pkv::kMinBlocks * pkv::block_positions(kv->elem());
+    // columns a multiple of the 8 XCDs: the tiles of one cached head land on one
+    const int64_t cols = p.shift >= 0 ? ((join ? p.slots : rows) + 7) / 8 * 8 : rows;
     return dispatch(kv, [&](auto hd, auto elem) -> int {
         hipLaunchKernelGGL((pkv_attend_kernel<decltype(hd)::value, decltype(elem)::value>),
-                           dim3((unsigned)a.n_head, (unsigned)rows), dim3(64), 0, ctx->stream, c, a);
+                           dim3((unsigned)cols, (unsigned)(kv->n_kv * p.tiles)), dim3(256), 0, ctx->stream, c, a);
+        if (join)
+            hipLaunchKernelGGL((pkv_join_kernel<decltype(hd)::value>), dim3((unsigned)a.n_head, (unsigned)rows),
+                               dim3(256), 0, ctx->stream, a);
         LLMQ_HIP(hipGetLastError());
         return LLMQ_OK;
     });
@@ -381,13 +779,14 @@ int llmq_pkv_fetch(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *k, float
 
 int64_t llmq_pkv_work_bytes(const llmq_pkv *kv, int64_t rows, int n_head) {
     if (!kv || rows < 0 || rows > 65535 || n_head <= 0 || n_head > 65535) return -1;
-    return 256;
+    if (n_head % kv->n_kv) return -1;
+    return pkv::work_of(pkv::plan_of(rows, n_head, kv->n_kv), rows, n_head, kv->hd).bytes;
 }
 
 int llmq_pkv_attend(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q, int64_t ldq,
                     int64_t rows, int n_head, const int32_t *len, const int32_t *table, int64_t width, float scale,
                     float cap, const float *slopes, void *work, int64_t work_bytes) {
-    Attend a{out, ldo, q, nullptr, nullptr, ldq, len, n_head, scale, cap, slopes};
+    Attend a{out, ldo, q, nullptr, nullptr, ldq, len, n_head, scale, cap, slopes, 0, 0, 0, nullptr, nullptr, nullptr};
     return attend("pkv_attend", ctx, kv, layer, a, rows, table, width, work, work_bytes);
 }
 
@@ -395,7 +794,7 @@ int llmq_pkv_step(llmq_ctx *ctx, llmq_pkv *kv, int layer, float *out, int64_t ld
                   const float *v, int64_t ld, int64_t rows, int n_head, const int32_t *pos, const int32_t *table,
                   int64_t width, float scale, float cap, const float *slopes, void *work, int64_t work_bytes) {
     LLMQ_REQUIRE((k && v) || rows == 0, "pkv_step: null argument");
-    Attend a{out, ldo, q, k, v, ld, pos, n_head, scale, cap, slopes};
+    Attend a{out, ldo, q, k, v, ld, pos, n_head, scale, cap, slopes, 0, 0, 0, nullptr, nullptr, nullptr};
     return attend("pkv_step", ctx, kv, layer, a, rows, table, width, work, work_bytes);
 }
 

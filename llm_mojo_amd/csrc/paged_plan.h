@@ -42,4 +42,53 @@ PKV_HD int64_t clamp_len(int64_t len, int64_t width, int page) {
     return len < 0 ? 0 : (len > most ? most : len);
 }
 
+// How a call's rows are split over workgroups.  A workgroup takes up to 8 of
+// the query heads of a cached head (`tiles` of them cover the group).  Up to kPlanRows rows,
+// the blocks of all rows are dealt into splits of one size, the least that
+// leaves at most 2^shift splits' worth of whole ones (and kMinBlocks, a
+// block a wave): a long row gets many, a short one one, and there are never
+// more than `slots`.  More rows fill the card by themselves and are not split (shift -1).
+constexpr int kWaves = 4;        // of a workgroup, each taking every kWaves-th block
+constexpr int kMinBlocks = 4;    // blocks of the smallest split
+constexpr int kPlanRows = 256;   // rows whose lengths a wave holds at once
+constexpr int kWorkgroups = 1024;  // aimed at, over all heads
+
+struct Plan {
+    int tiles, shift;
+    int64_t slots;
+};
+
+PKV_HD Plan plan_of(int64_t rows, int n_head, int n_kv) {
+    Plan p;
+    p.tiles = (n_head / n_kv + 7) / 8;
+    p.shift = -1;
+    p.slots = rows;
+    if (rows > kPlanRows) return p;
+    p.shift = 0;
+    while (((int64_t)n_kv * p.tiles << (p.shift + 1)) <= kWorkgroups) p.shift++;
+    p.slots = rows + ((int64_t)1 << p.shift);
+    return p;
+}
+
+// Blocks a split, given those of all rows; and splits of a row of nb blocks (at least one, for the row's output).
+PKV_HD int64_t split_blocks(int64_t total, int shift) {
+    const int64_t n = (total >> shift) + 1;
+    return n < kMinBlocks ? kMinBlocks : (n > 0x7fffffff ? 0x7fffffff : n);
+}
+PKV_HD uint32_t row_splits(uint32_t nb, uint32_t blocks) { return nb <= blocks ? 1 : (nb - 1) / blocks + 1; }
+
+// Byte offsets of a call's workspace: per row the first split and their
+// number, per (split, head) the reference and sum of its exponentials, and its sums of values.
+struct Work {
+    int64_t ml, sums, bytes;
+};
+PKV_HD Work work_of(const Plan &p, int64_t rows, int n_head, int hd) {
+    Work w;
+    const int64_t slots = p.shift < 0 ? 0 : p.slots;
+    w.ml = (rows * 8 + 255) & ~(int64_t)255;
+    w.sums = w.ml + ((slots * n_head * 8 + 255) & ~(int64_t)255);
+    w.bytes = w.sums + slots * n_head * hd * 4;
+    return w;
+}
+
 }  // namespace pkv
