@@ -21,6 +21,7 @@ import math
 import torch
 
 own = False
+opened = []
 
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -174,13 +175,20 @@ def logit_inputs(case, g):
     return s
 
 
+def library():
+    """The package and the one context that a program has: every state's calls go to one stream."""
+    if not opened:
+        import llm_mojo_amd as lm
+
+        opened.append((lm, lm.Context(0, torch.cuda.current_stream())))
+    return opened[0]
+
+
 def prepare(case, seed):
     g = generator(seed)
     s = {"case": case}
     if own:
-        import llm_mojo_amd as lm
-
-        s["lm"], s["ctx"] = lm, lm.Context(0, torch.cuda.current_stream())
+        s["lm"], s["ctx"] = library()
     if case["kind"] in ("step", "store"):
         kv, hd, page = case["kv"], case["hd"], case["page"]
         s["length"], s["table"], n_pages = paged(case, seed, g)
