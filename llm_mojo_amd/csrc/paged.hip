@@ -24,6 +24,8 @@ struct llmq_pkv {
 
 namespace {
 
+constexpr int B = pkv::kBlock;
+
 // One layer of a cache as a kernel takes it.
 struct Layer {
     uint8_t *k, *v;
@@ -32,6 +34,10 @@ struct Layer {
     int64_t width, pages;
     int page, n_kv;
 };
+
+// int8 codes are kept plus 128: 0x64 above such a byte is the float16 1024 +
+// code + 128, which is how the attention widens them.
+constexpr int kBias = 128;
 
 // A head's row (position 0 of its page) in units of positions.
 __device__ __forceinline__ int64_t head_row(const Layer &c, int page, int head) {
@@ -65,40 +71,58 @@ __device__ __forceinline__ uint16_t half_bits(float x) {
     return __half_as_ushort(__float2half_rn(lim));
 }
 
-// One wave writes the key and value row of (token, head).
+// A row's codes (int8 with kBias, or float16 bits) and scale, dimensions lane + 64 i.
 template <int HD, int ELEM>
-__device__ __forceinline__ void store_row(const Layer &c, int page, int off, int head, const float *k, const float *v,
-                                          int lane) {
+__device__ __forceinline__ float encode_row(const float (&x)[HD / 64], int (&code)[HD / 64]) {
+    if constexpr (ELEM == 1) {
+        const float s = quant_row<HD>(x, code);
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) code[i] += kBias;
+        return s;
+    } else {
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) code[i] = half_bits(x[i]);
+        return 1.0f;
+    }
+}
+
+// One wave writes the key and value row of (token, head); the codes stay with it.
+template <int HD, int ELEM>
+struct NewRow {
+    int k[HD / 64], v[HD / 64];
+    float ks, vs;
+};
+template <int HD, int ELEM>
+__device__ __forceinline__ NewRow<HD, ELEM> store_row(const Layer &c, int page, int off, int head, const float *k,
+                                                      const float *v, int lane) {
     const int64_t row = head_row(c, page, head) + off;
-    const int B = pkv::block_positions(ELEM), blk = off / B;
-    const int64_t vrow = (head_row(c, page, head) + (int64_t)blk * B) * HD;  // the block's first element
-    const int slot = pkv::value_slot(ELEM, off % B);
+    const int64_t vrow = (head_row(c, page, head) + off / B * B) * HD;  // the block's first element
+    const int slot = pkv::value_slot(off % B);
     float kx[HD / 64], vx[HD / 64];
 #pragma unroll
     for (int i = 0; i < HD / 64; i++) {
         kx[i] = k[lane + 64 * i];
         vx[i] = v[lane + 64 * i];
     }
-    if constexpr (ELEM == 1) {
-        int kc[HD / 64], vc[HD / 64];
-        const float s = quant_row<HD>(kx, kc), t = quant_row<HD>(vx, vc);
+    NewRow<HD, ELEM> x;
+    x.ks = encode_row<HD, ELEM>(kx, x.k);
+    x.vs = encode_row<HD, ELEM>(vx, x.v);
 #pragma unroll
-        for (int i = 0; i < HD / 64; i++) {
-            c.k[row * HD + lane + 64 * i] = (uint8_t)kc[i];
-            c.v[vrow + (int64_t)(lane + 64 * i) * B + slot] = (uint8_t)vc[i];
-        }
-        if (lane == 0) {
-            c.ks[row] = s;
-            c.vs[row] = t;
-        }
-    } else {
-        uint16_t *ck = reinterpret_cast<uint16_t *>(c.k), *cv = reinterpret_cast<uint16_t *>(c.v);
-#pragma unroll
-        for (int i = 0; i < HD / 64; i++) {
-            ck[row * HD + lane + 64 * i] = half_bits(kx[i]);
-            cv[vrow + (int64_t)(lane + 64 * i) * B + slot] = half_bits(vx[i]);
+    for (int i = 0; i < HD / 64; i++) {
+        const int64_t kat = row * HD + lane + 64 * i, vat = vrow + (int64_t)(lane + 64 * i) * B + slot;
+        if constexpr (ELEM == 1) {
+            c.k[kat] = (uint8_t)x.k[i];
+            c.v[vat] = (uint8_t)x.v[i];
+        } else {
+            reinterpret_cast<uint16_t *>(c.k)[kat] = (uint16_t)x.k[i];
+            reinterpret_cast<uint16_t *>(c.v)[vat] = (uint16_t)x.v[i];
         }
     }
+    if (ELEM == 1 && lane == 0) {
+        c.ks[row] = x.ks;
+        c.vs[row] = x.vs;
+    }
+    return x;
 }
 
 // Element (lane + 64 i) of a cached key / value row.
@@ -106,15 +130,14 @@ template <int HD, int ELEM>
 __device__ __forceinline__ void load_row(const Layer &c, int page, int off, int head, float (&k)[HD / 64],
                                          float (&v)[HD / 64], int lane) {
     const int64_t row = head_row(c, page, head) + off;
-    const int B = pkv::block_positions(ELEM), blk = off / B;
-    const int64_t vrow = (head_row(c, page, head) + (int64_t)blk * B) * HD;
-    const int slot = pkv::value_slot(ELEM, off % B);
+    const int64_t vrow = (head_row(c, page, head) + off / B * B) * HD;
+    const int slot = pkv::value_slot(off % B);
 #pragma unroll
     for (int i = 0; i < HD / 64; i++) {
         const int d = lane + 64 * i;
         if constexpr (ELEM == 1) {
-            k[i] = (float)(int8_t)c.k[row * HD + d] * c.ks[row];
-            v[i] = (float)(int8_t)c.v[vrow + (int64_t)d * B + slot] * c.vs[row];
+            k[i] = (float)((int)c.k[row * HD + d] - kBias) * c.ks[row];
+            v[i] = (float)((int)c.v[vrow + (int64_t)d * B + slot] - kBias) * c.vs[row];
         } else {
             k[i] = __half2float(__ushort_as_half(reinterpret_cast<const uint16_t *>(c.k)[row * HD + d]));
             v[i] = __half2float(
@@ -166,10 +189,10 @@ struct Attend {
     int n_head;
     float scale, cap;
     const float *slopes;
-    int rows, tiles, shift;
-    int2 *meta;    // [row]: first split, number of splits
-    float2 *ml;    // [split][head]: reference (log2), sum
-    float *sums;   // [split][head][hd]
+    int rows, tiles, columns;  // columns 0: a workgroup a row
+    int2 *meta;   // [row]: first and last slot
+    float2 *ml;   // [slot][head]: reference (log2), sum
+    float *sums;  // [slot][head][hd]
 };
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -188,8 +211,6 @@ __device__ __forceinline__ h8 halves(uint32_t a, uint32_t b) {
         h8 v;
     } r;
     const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
     r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
     r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
     r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
@@ -199,13 +220,32 @@ __device__ __forceinline__ h8 halves(uint32_t a, uint32_t b) {
     return r.v;
 }
 
-__device__ __forceinline__ h8 as_h8(const uint4 &x) {
+__device__ __forceinline__ h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     union {
-        uint4 u;
+        uint32_t u[4];
         h8 v;
     } r;
-    r.u = x;
+    r.u[0] = a;
+    r.u[1] = b;
+    r.u[2] = c;
+    r.u[3] = d;
     return r.v;
+}
+
+// tanh without branches, to 2^-23 of 1: ref_tanhf's polynomial below 0.625,
+// 1 - 2 / (e^(2|y|) + 1) above.
+__device__ __forceinline__ float tanh_select(float y) {
+    const float a = fabsf(y), s = y * y;
+    float p = 0.002148991f;
+    p = fmaf(p, s, -0.00818467f);
+    p = fmaf(p, s, 0.021704003f);
+    p = fmaf(p, s, -0.053947456f);
+    p = fmaf(p, s, 0.13333212f);
+    p = fmaf(p, s, -0.3333333f);
+    p = fmaf(p * s, a, a);
+    const float e = __builtin_amdgcn_exp2f(a * (2.0f * kLog2e));
+    const float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    return copysignf(a < 0.625f ? p : t, y);
 }
 
 // Maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
@@ -222,63 +262,80 @@ __device__ __forceinline__ float quarters_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x),
+                   hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 __device__ __forceinline__ int64_t row_len(const Layer &c, const Attend &a, int64_t r) {
     const int64_t n = a.len[r];
     return pkv::clamp_len(a.k ? n + 1 : n, c.width, c.page);
 }
 
-// Which part of which row workgroup column `slot` takes; every wave finds it
-// by itself from the rows' lengths (a.rows <= kPlanRows).
+// The segment of a slot, blocks b0 .. b1 - 1 of a row (none: b0 = b1 = 0);
+// every wave finds it by itself from the rows' lengths (a.rows <= kPlanRows).
 struct Part {
-    int row, split, count, first;  // row -1: nothing
-    int64_t blocks;                // blocks a split
+    int row, b0, b1;
 };
-__device__ __forceinline__ Part find_part(const Layer &c, const Attend &a, int B, int slot, int lane) {
+__device__ __forceinline__ Part find_part(const Layer &c, const Attend &a, uint32_t slot, int lane) {
     constexpr int N = pkv::kPlanRows / 64;
-    uint32_t nb[N];
-    int64_t total = 0;
+    uint32_t nb[N], end[N], total = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int r = 64 * i + lane;
         nb[i] = r < a.rows ? (uint32_t)((row_len(c, a, r) + B - 1) / B) : 0;
-        total += nb[i];
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    Part p;
-    p.blocks = pkv::split_blocks(total, a.shift);
-    p.row = -1;
-    uint32_t before = 0;
+    for (int i = 0; i < N; i++) {  // ends in the line of all blocks
+        end[i] = nb[i];
+        if (64 * i >= a.rows) break;
+        if (a.rows > 1)
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t up = __shfl_up(end[i], o);
+                if (lane >= o) end[i] += up;
+            }
+        end[i] += total;
+        total = __shfl(end[i], a.rows > 1 ? 63 : 0);
+    }
+    const uint32_t per = pkv::column_blocks(total, a.columns);
+    Part p{0, 0, 0};
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if (64 * i >= a.rows) break;
-        const uint32_t mine = 64 * i + lane < a.rows ? pkv::row_splits(nb[i], (uint32_t)p.blocks) : 0;
-        uint32_t incl = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t up = __shfl_up(incl, o);
-            if (lane >= o) incl += up;
-        }
-        const uint32_t all = __shfl(incl, 63);
-        if (p.row < 0 && (uint32_t)slot < before + all) {
-            const int at = __popcll(__ballot(before + incl <= (uint32_t)slot));  // < 64
-            const uint32_t end = __shfl(incl, at), n = __shfl(mine, at);
-            p.row = 64 * i + at;
-            p.count = (int)n;
-            p.first = (int)(before + end - n);
-            p.split = slot - p.first;
-        }
-        before += all;
+        const int r = 64 * i + lane;
+        p.row += __popcll(__ballot(r < a.rows && r + 1 + end[i] / per <= slot));
     }
+    if (p.row >= a.rows) return p;
+    uint32_t e = 0, n = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t x = __shfl(end[i], p.row & 63), y = __shfl(nb[i], p.row & 63);
+        if (i == p.row >> 6) e = x, n = y;
+    }
+    const uint64_t begin = e - n, column = (uint64_t)(slot - p.row) * per;
+    const uint64_t lo = column > begin ? column : begin, hi = e < column + per ? e : column + per;
+    if (lo >= hi) return p;
+    p.b0 = (int)(lo - begin);
+    p.b1 = (int)(hi - begin);
     return p;
 }
 
-// Attention of one token over a row's pages, or a split of it: 4 waves, up to
-// 8 query heads of one cached head, on the fp16 matrix cores.
+struct Float8 {
+    float x[8];
+} __attribute__((packed, aligned(4)));
+
+// A table entry by a scalar load, which does not wait for the vector loads in flight.
+__device__ __forceinline__ int table_at(const int32_t *p) {
+    return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p;
+}
+
+// Attention of one token over what a column has of the rows: up to 8 query
+// heads of one cached head, on the fp16 matrix cores.
 //
 // Scores: K (16 positions x 32 dimensions) times the queries as 16 columns,
 // columns 0-7 their float16 roundings and 8-15 what those leave times 2^11
-// (22 bits in all; the keys are exact), so column n and n ^ 8 add up to a
+// (22 bits in all; the keys are exact), so columns n and n ^ 8 add up to a
 // score, in lane n for positions 4 (lane / 16) + 0..3 of the tile.  Values:
 // the weights are already where the second product wants its rows: row n
 // holds head n's weights as float16, row n ^ 8 what is left times 2^11, and
@@ -287,122 +344,168 @@ __device__ __forceinline__ Part find_part(const Layer &c, const Attend &a, int B
 // power of two near the largest scale so far.
 //
 // The reference of a head's exponentials is moved (and the sums rescaled)
-// only when a score passes it by 2^6, which is rare after the first blocks.
-// Each wave keeps its own and reads every fourth block; the four are put
+// only when a score passes it by 4, which is rare after the first blocks.
+// Each wave keeps its own and reads every fourth block; they are put
 // together through LDS.  A wave's next keys are on their way while it forms
 // the weights, its next values while it scores.
 template <int HD, int ELEM>
-__global__ __launch_bounds__(256, 2) void pkv_attend_kernel(Layer c, Attend a) {
-    constexpr int B = ELEM == 1 ? 64 : 32, NT = B / 16, NC = HD * ELEM / 64, NF = HD / 32, ND = HD / 16;
-    constexpr int kBlock = HD * 64;  // bytes of a block's keys, and of its values
-    __shared__ __align__(16) _Float16 qp[16][HD];
-    __shared__ float qexp[8];
+__global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c, Attend a) {
+    constexpr int NT = B / 16, NC = HD * ELEM / 64, NF = HD / 32, ND = HD / 16, NV = 2 * ELEM;
+    constexpr int kBytes = B * HD * ELEM;  // of a block's keys, and of its values
+    __shared__ __align__(16) uint8_t fresh[2][HD * ELEM];  // the new token's key and value
     __shared__ float2 wml[pkv::kWaves][8];
     __shared__ float wsum[pkv::kWaves][8][HD];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15,
+              q = lane >> 4;
     const int kvh = blockIdx.y / a.tiles, G = a.n_head / c.n_kv, t0 = blockIdx.y % a.tiles * 8;
     const int h0 = kvh * G + t0, hn = min(8, G - t0);
-
-    Part part;
-    if (a.shift >= 0) {
-        part = find_part(c, a, B, blockIdx.x, lane);
-        if (part.row < 0) return;  // the same for the whole workgroup
-    } else {
-        part = Part{(int)blockIdx.x, 0, 1, 0, 0x7fffffff};
-    }
-    const int64_t r = __builtin_amdgcn_readfirstlane(part.row);
-    const int32_t *table = c.table + r * c.width;
-    const int64_t len = row_len(c, a, r);
-    const int nb = (int)((len + B - 1) / B);
-    const int64_t e64 = (part.split + 1) * part.blocks;
-    const int b0 = __builtin_amdgcn_readfirstlane((int)(part.split * part.blocks)),
-              b1 = __builtin_amdgcn_readfirstlane((int)(e64 < nb ? e64 : nb));
-    const int count = __builtin_amdgcn_readfirstlane(part.count);
-
-    // the new token's rows, by the workgroups whose split ends with it (the
-    // tiles of a group write the same bytes, and each reads its own)
-    if (a.k && len > 0 && b1 == nb && w == pkv::kWaves - 1) {
-        const int64_t p = len - 1;
-        const int page = a.len[r] == p ? pkv::page_of(table, c.width, c.page, c.pages, p) : -1;
-        if (page >= 0)
-            store_row<HD, ELEM>(c, page, (int)(p % c.page), kvh, a.k + r * a.ldq + kvh * HD, a.v + r * a.ldq + kvh * HD,
-                                lane);
-    }
-    // queries to their planes: heads 2 w and 2 w + 1
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int h = 2 * w + i;
-        float x[HD / 64], m = 0.0f;
-#pragma unroll
-        for (int d = 0; d < HD / 64; d++) {
-            x[d] = h < hn ? a.q[r * a.ldq + (int64_t)(h0 + h) * HD + lane + 64 * d] : 0.0f;
-            m = fmaxf(m, fabsf(x[d]));
-        }
-        m = llmq_wave_max_all(m);
-        const int e = m > 0.0f ? (int)(__float_as_uint(m) >> 23) - 127 : 0;
-#pragma unroll
-        for (int d = 0; d < HD / 64; d++) {
-            const float y = ldexpf(x[d], -e);
-            const _Float16 hi = (_Float16)y;
-            qp[h][lane + 64 * d] = hi;
-            qp[h + 8][lane + 64 * d] = (_Float16)((y - (float)hi) * 2048.0f);
-        }
-        if (lane == 0) qexp[h] = ldexpf(a.scale, e);
-    }
-    __syncthreads();
-    h8 qf[NF];
-#pragma unroll
-    for (int f = 0; f < NF; f++) {
-        const int d = ELEM == 1 ? (f >> 1) * 64 + q * 16 + (f & 1) * 8 : f * 32 + q * 8;
-        qf[f] = *reinterpret_cast<const h8 *>(&qp[n][d]);
-    }
-    const bool low = n >= 8;
-    const float mul = qexp[n & 7];
-    const float own = low ? 0x1p-11f : 1.0f, oth = low ? 1.0f : 0x1p-11f;  // a score from the two columns
-    const float wg = low ? 2048.0f : 1.0f, wr = low ? -2048.0f : 0.0f;     // a weight to its row's share
-    const float slope = a.slopes && (n & 7) < hn ? a.slopes[h0 + (n & 7)] : 0.0f;
-    const bool bias = a.slopes != nullptr;
-
     const int bpp = c.page / B;
-    const int64_t head_bytes = (int64_t)c.page * HD * ELEM;
-    const uint32_t koff = (uint32_t)(n * HD * ELEM + q * 16), voff = (uint32_t)(n * 64 + q * 16);
-    struct Where {
-        const uint8_t *k, *v;
-        const float *ks, *vs;
-        int live;
-    };
-    auto where = [&](int b) {
-        Where x;
-        const int p = __builtin_amdgcn_readfirstlane(b / bpp), o = b - p * bpp;
-        const int page = __builtin_amdgcn_readfirstlane(table[p]);
+    const bool low = n >= 8;
+
+    int64_t r = blockIdx.x;
+    int b0 = 0, b1 = 0;
+    if (a.columns) {
+        const Part part = find_part(c, a, blockIdx.x, lane);
+        r = __builtin_amdgcn_readfirstlane(part.row);
+        b0 = __builtin_amdgcn_readfirstlane(part.b0);
+        b1 = __builtin_amdgcn_readfirstlane(part.b1);
+        if (b0 == b1) return;  // the same for the whole workgroup
+    }
+    const int32_t *table = c.table + r * c.width;
+    const int64_t len = uniform64(row_len(c, a, r));
+    const int nb = (int)((len + B - 1) / B);
+    if (!a.columns) b1 = nb;
+    const bool whole = b0 == 0 && b1 == nb;
+
+    // the lane's part of its column's query: the column's plane of its dimensions
+    float x[NF][8];
+    {
+        const float *src = a.q + r * a.ldq + (int64_t)(h0 + min(n & 7, hn - 1)) * HD;
+#pragma unroll
+        for (int f = 0; f < NF; f++)
+            *reinterpret_cast<Float8 *>(x[f]) = *reinterpret_cast<const Float8 *>(
+                src + (ELEM == 1 ? (f >> 1) * 64 + q * 16 + (f & 1) * 8 : f * 32 + q * 8));
+    }
+    // a block: its page (page 0 in the place of one that is none, with no live positions) and its rows there
+    int b = b0 + w, pi = b / bpp, off = b - pi * bpp;
+    uint32_t kr[NT * NC][4], vr[ND][NV];
+    v4f ks[NT], vs[NT];
+    int64_t at = 0;  // the block's first row
+    int bytes = kBytes;  // of its keys, and of its values: none of a page that is none, whose loads give zeros
+    auto find = [&]() -> int {
+        const int page = table_at(table + __builtin_amdgcn_readfirstlane(pi));
         const bool ok = page >= 0 && page < c.pages;
-        const int64_t hr = (int64_t)(ok ? page : 0) * c.n_kv + kvh;
-        x.k = c.k + hr * head_bytes + (int64_t)o * kBlock;
-        x.v = c.v + hr * head_bytes + (int64_t)o * kBlock;
-        x.ks = ELEM == 1 ? c.ks + hr * c.page + o * B : nullptr;
-        x.vs = ELEM == 1 ? c.vs + hr * c.page + o * B : nullptr;
+        at = uniform64(((int64_t)(ok ? page : 0) * c.n_kv + kvh) * c.page + off * B);
+        bytes = __builtin_amdgcn_readfirstlane(ok ? kBytes : 0);
         const int64_t left = len - (int64_t)b * B;
-        x.live = ok ? (int)(left < B ? left : B) : 0;
-        return x;
+        return __builtin_amdgcn_readfirstlane(ok ? (int)(left < B ? left : B) : 0);
     };
-    uint4 kr[NT * NC], vr[ND];
-    float4 ks[NT], vs[NT];
-    auto load_k = [&](const Where &x) {
+    auto load_k = [&]() {
+        const auto rk = llmq_rsrc(c.k + at * HD * ELEM, bytes);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int i = 0; i < NC; i++)
-                kr[t * NC + i] = *reinterpret_cast<const uint4 *>(x.k + koff + t * 16 * HD * ELEM + i * 64);
+            for (int i = 0; i < NC; i++) {
+                const auto y = __builtin_amdgcn_raw_buffer_load_b128(rk, n * HD * ELEM + q * 16,
+                                                                     t * 16 * HD * ELEM + i * 64, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) kr[t * NC + i][e] = y[e];
+            }
+        if constexpr (ELEM == 1) {
+            const auto rs = llmq_rsrc(c.ks + at, bytes < 4 * B ? bytes : 4 * B);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                ks[t] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * q, 64 * t, 0));
+        }
+    };
+    auto load_v = [&]() {
+        const auto rv = llmq_rsrc(c.v + at * HD * ELEM, bytes);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const int vo = (n * B + q * 8) * ELEM, so = d * 16 * B * ELEM;
             if constexpr (ELEM == 1) {
-                ks[t] = *reinterpret_cast<const float4 *>(x.ks + 16 * t + 4 * q);
-                vs[t] = *reinterpret_cast<const float4 *>(x.vs + 16 * t + 4 * q);
+                const auto y = __builtin_amdgcn_raw_buffer_load_b64(rv, vo, so, 0);
+                vr[d][0] = y[0];
+                vr[d][1] = y[1];
+            } else {
+                const auto y = __builtin_amdgcn_raw_buffer_load_b128(rv, vo, so, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) vr[d][e] = y[e];
             }
         }
-    };
-    auto load_v = [&](const Where &x) {
+        if constexpr (ELEM == 1) {
+            const auto rs = llmq_rsrc(c.vs + at, bytes < 4 * B ? bytes : 4 * B);
 #pragma unroll
-        for (int d = 0; d < ND; d++) vr[d] = *reinterpret_cast<const uint4 *>(x.v + voff + d * 1024);
+            for (int t = 0; t < NT; t++)
+                vs[t] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * q, 64 * t, 0));
+        }
     };
+    // the first block's rows are asked for before the query is taken apart
+    int live = 0;
+    if (b < b1) {
+        live = find();
+        load_k();
+        load_v();
+    }
+    h8 qf[NF];
+    float mul;
+    {
+        float m = 0.0f;
+#pragma unroll
+        for (int f = 0; f < NF; f++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if ((n & 7) >= hn) x[f][i] = 0.0f;
+                m = fmaxf(m, fabsf(x[f][i]));
+            }
+        m = quarters_max(m);
+        const int e = m > 0.0f ? (int)(__float_as_uint(m) >> 23) - 127 : 0;
+        mul = ldexpf(a.scale, e);
+#pragma unroll
+        for (int f = 0; f < NF; f++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float y = ldexpf(x[f][i], -e);
+                const _Float16 hi = (_Float16)y;
+                qf[f][i] = low ? (_Float16)((y - (float)hi) * 2048.0f) : hi;
+            }
+    }
+    const float own = low ? 0x1p-11f : 1.0f, oth = low ? 1.0f : 0x1p-11f;  // a score from the two columns
+    const float wg = low ? 2048.0f : 1.0f, wr = low ? -2048.0f : 0.0f;     // a weight to its row's share
+    const float icap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const bool bias = a.slopes != nullptr;
+    float slope = bias && (n & 7) < hn ? a.slopes[h0 + (n & 7)] : 0.0f;
+    asm volatile("" : "+v"(slope));  // waited for here, not behind the loop's loads
+
+    // the new token's row: stored by the wave whose last block holds it
+    // (the tiles of a group store the same bytes), which puts it into
+    // that block as it came from memory
+    int fb = -1;
+    float fks = 0.0f, fvs = 0.0f;
+    if (a.k && len > 0 && b1 == nb && (nb - 1 - b0) % pkv::kWaves == w) {
+        const int64_t p = len - 1;
+        const int page = a.len[r] == p ? pkv::page_of(table, c.width, c.page, c.pages, p) : -1;
+        if (page >= 0) {
+            const int64_t src = r * a.ldq + kvh * HD;
+            const NewRow<HD, ELEM> y =
+                store_row<HD, ELEM>(c, page, (int)(p % c.page), kvh, a.k + src, a.v + src, lane);
+#pragma unroll
+            for (int i = 0; i < HD / 64; i++) {
+                if constexpr (ELEM == 1) {
+                    fresh[0][lane + 64 * i] = (uint8_t)y.k[i];
+                    fresh[1][lane + 64 * i] = (uint8_t)y.v[i];
+                } else {
+                    reinterpret_cast<uint16_t *>(fresh[0])[lane + 64 * i] = (uint16_t)y.k[i];
+                    reinterpret_cast<uint16_t *>(fresh[1])[lane + 64 * i] = (uint16_t)y.v[i];
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            fks = y.ks;
+            fvs = y.vs;
+            fb = nb - 1;
+        }
+    }
+    fb = __builtin_amdgcn_readfirstlane(fb);
 
     v4f acc[ND];
 #pragma unroll
@@ -410,18 +513,46 @@ __global__ __launch_bounds__(256, 2) void pkv_attend_kernel(Layer c, Attend a) {
     float ref = kLowest, ref2 = kLowest, l = 0.0f;  // ref2 = ref log2 e, rounded once
     int ve = ELEM == 1 ? -100 : 0;                   // the weights' power of two
 
-    int b = b0 + w;
-    Where cur{};
-    if (b < b1) {
-        cur = where(b);
-        load_k(cur);
-        load_v(cur);
-    }
-    for (; b < b1; b += pkv::kWaves) {
-        const int live = cur.live, j0 = b * B;
-        const bool more = b + pkv::kWaves < b1;
-        Where next{};
-        if (more) next = where(b + pkv::kWaves);
+    // one block; LAST: the wave's last, which may hold the new token and the
+    // row's end (the others are whole, or in a page that is none)
+    auto block = [&](auto last) {
+        constexpr bool LAST = decltype(last)::value;
+        const int j0 = b * B, have = live;
+        if (LAST && b == fb) {
+            const int o = (int)(len - 1) - j0, ft = o >> 4, fq = (o >> 2) & 3, fi = o & 3;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                if (t != ft) continue;
+                if (n == (o & 15))
+#pragma unroll
+                    for (int i = 0; i < NC; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            kr[t * NC + i][e] =
+                                *reinterpret_cast<const uint32_t *>(&fresh[0][i * 64 + q * 16 + 4 * e]);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (ELEM == 1 && i == fi && q == fq) {
+                        ks[t][i] = fks;
+                        vs[t][i] = fvs;
+                    }
+            }
+            const int word = (ft * 4 + fi) * ELEM / 4, sh = (ft * 4 + fi) * ELEM % 4 * 8;
+            const uint32_t keep = ~((ELEM == 1 ? 0xffu : 0xffffu) << sh);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const uint32_t code = ELEM == 1 ? fresh[1][16 * d + n]
+                                                : reinterpret_cast<const uint16_t *>(fresh[1])[16 * d + n];
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+                    if (i == word && q == fq) vr[d][i] = (vr[d][i] & keep) | code << sh;
+            }
+        }
+        if constexpr (!LAST) {
+            b += pkv::kWaves;
+            for (off += pkv::kWaves; off >= bpp; off -= bpp) pi++;
+            live = find();
+        }
         // scores
         v4f s[NT];
 #pragma unroll
@@ -429,67 +560,67 @@ __global__ __launch_bounds__(256, 2) void pkv_attend_kernel(Layer c, Attend a) {
             s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < NC; i++) {
-                const uint4 x = kr[t * NC + i];
+                const uint32_t *y = kr[t * NC + i];
                 if constexpr (ELEM == 1) {
-                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x.x, x.y), qf[2 * i], s[t], 0, 0, 0);
-                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x.z, x.w), qf[2 * i + 1], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(y[0], y[1]), qf[2 * i], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(y[2], y[3]), qf[2 * i + 1], s[t], 0, 0, 0);
                 } else {
-                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(x), qf[i], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(y[0], y[1], y[2], y[3]), qf[i], s[t], 0, 0,
+                                                                  0);
                 }
             }
         }
-        float sv[NT * 4], vsc[NT * 4];
+        float sv[NT * 4];
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float x = s[t][i] * own + llmq_dppf<0x128>(s[t][i]) * oth;  // row_ror:8
-                if constexpr (ELEM == 1) {
-                    x *= reinterpret_cast<const float *>(&ks[t])[i];
-                    vsc[4 * t + i] = reinterpret_cast<const float *>(&vs[t])[i];
-                }
-                sv[4 * t + i] = x * mul;
+                float y = s[t][i] * own + llmq_dppf<0x128>(s[t][i]) * oth;  // row_ror:8
+                if constexpr (ELEM == 1) y *= ks[t][i];
+                sv[4 * t + i] = y * mul;
             }
-        if (more) load_k(next);
+        if constexpr (!LAST) load_k();
         if (a.cap > 0.0f)
 #pragma unroll
-            for (int i = 0; i < NT * 4; i++) sv[i] = a.cap * ref_tanhf(sv[i] / a.cap);
+            for (int i = 0; i < NT * 4; i++) sv[i] = a.cap * tanh_select(sv[i] * icap);
         if (bias) {
             const float base = (float)(j0 + 4 * q - (len - 1));
 #pragma unroll
             for (int i = 0; i < NT * 4; i++) sv[i] = fmaf(slope, base + (float)(16 * (i >> 2) + (i & 3)), sv[i]);
         }
-        if (live < B) {  // the row's end, or a page that is none
+        if (!LAST && have == 0)
+#pragma unroll
+            for (int i = 0; i < NT * 4; i++) sv[i] = -INFINITY;
+        if (LAST && have < B) {
 #pragma unroll
             for (int i = 0; i < NT * 4; i++) {
-                const bool in = 16 * (i >> 2) + 4 * q + (i & 3) < live;
+                const bool in = 16 * (i >> 2) + 4 * q + (i & 3) < have;
                 sv[i] = in ? sv[i] : -INFINITY;
-                if constexpr (ELEM == 1) vsc[i] = in ? vsc[i] : 0.0f;
+                if constexpr (ELEM == 1) vs[i >> 2][i & 3] = in ? vs[i >> 2][i & 3] : 0.0f;
             }
             if constexpr (ELEM == 2) {  // what lies there may be NaN
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    uint32_t *u = reinterpret_cast<uint32_t *>(&vr[d]);
+                for (int i = 0; i < 4; i++) {
+                    const int p = 16 * (i >> 1) + 4 * q + 2 * (i & 1);
+                    const uint32_t keep = p + 1 < have ? 0xffffffffu : (p < have ? 0xffffu : 0u);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int p = 16 * (i >> 1) + 4 * q + 2 * (i & 1);
-                        u[i] &= p + 1 < live ? 0xffffffffu : (p < live ? 0xffffu : 0u);
-                    }
+                    for (int d = 0; d < ND; d++) vr[d][i] &= keep;
                 }
             }
         }
-        float mx = sv[0], vm = 0.0f;
+        float mx = sv[0];
 #pragma unroll
         for (int i = 1; i < NT * 4; i++) mx = fmaxf(mx, sv[i]);
         mx = quarters_max(mx);
         int nve = ve;
         if constexpr (ELEM == 1) {
+            float vm = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NT * 4; i++) vm = fmaxf(vm, vsc[i]);
+            for (int i = 0; i < NT * 4; i++) vm = fmaxf(vm, vs[i >> 2][i & 3]);
             vm = quarters_max(vm);
             nve = max(ve, (int)(__float_as_uint(vm) >> 23) - 127);
         }
-        if (__any(mx > ref + 4.0f || nve > ve)) {  // 4 log2 e < 6
+        if (__any(mx > ref + 4.0f || nve > ve)) {  // exponentials stay below 2^6
             const float to = fmaxf(ref, mx), to2 = to * kLog2e;
             const float f = ref == to ? 1.0f : exp2f(ref2 - to2), fl = ldexpf(f, ve - nve);
             ref = to;
@@ -498,51 +629,49 @@ __global__ __launch_bounds__(256, 2) void pkv_attend_kernel(Layer c, Attend a) {
             l *= f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x = __shfl(fl, 4 * q + i);  // of row 4 q + i
+                const float y = __shfl(fl, 4 * q + i);  // of row 4 q + i
 #pragma unroll
-                for (int d = 0; d < ND; d++) acc[d][i] *= x;
+                for (int d = 0; d < ND; d++) acc[d][i] *= y;
             }
         }
         const float unit = ldexpf(1.0f, 8 - ve);
-        h8 wf[NT / 2];
+        h8 wf;
 #pragma unroll
         for (int i = 0; i < NT * 4; i++) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sv[i], kLog2e, -ref2));
             l += p;
-            const float x = ELEM == 1 ? p * (vsc[i] * unit) : p * unit;
-            const float hi = (float)(_Float16)x;
-            // row n: x rounded; row n ^ 8: what that leaves times 2^11 (exact)
-            wf[i >> 3][i & 7] = (_Float16)fmaf(hi, wr, x * wg);
+            const float y = ELEM == 1 ? p * (vs[i >> 2][i & 3] * unit) : p * unit;
+            const float hi = (float)(_Float16)y;
+            // row n: y rounded; row n ^ 8: what that leaves times 2^11 (exact)
+            wf[i] = (_Float16)fmaf(hi, wr, y * wg);
         }
         // values
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-            const uint4 x = vr[d];
-            if constexpr (ELEM == 1) {
-                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[0], halves(x.x, x.y), acc[d], 0, 0, 0);
-                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[1], halves(x.z, x.w), acc[d], 0, 0, 0);
-            } else {
-                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[0], as_h8(x), acc[d], 0, 0, 0);
-            }
+            const h8 y = ELEM == 1 ? halves(vr[d][0], vr[d][1])
+                                   : as_h8(vr[d][0], vr[d][1], vr[d][NV - 2], vr[d][NV - 1]);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, y, acc[d], 0, 0, 0);
         }
-        if (more) {
-            load_v(next);
-            cur = next;
-        }
-    }
-    // the four waves' results
+        if constexpr (!LAST) load_v();
+    };
+    while (b + pkv::kWaves < b1) block(std::false_type{});
+    if (b < b1) block(std::true_type{});
+    // the waves' results
     l = quarters_sum(l);
     if (lane < 8) wml[w][n] = make_float2(ref2, l);
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float x = acc[d][i], y = __shfl_xor(x, 32);  // rows 4 q + i and 4 q + i + 8
-            if (q < 2) wsum[w][4 * q + i][16 * d + n] = ldexpf(fmaf(y, 0x1p-11f, x), ve - 8);
+            const float y = acc[d][i], z = __shfl_xor(y, 32);  // rows 4 q + i and 4 q + i + 8
+            if (q < 2) wsum[w][4 * q + i][16 * d + n] = ldexpf(fmaf(z, 0x1p-11f, y), ve - 8);
         }
     __syncthreads();
-    if (tid == 0 && blockIdx.y == 0 && part.split == 0 && a.shift >= 0) a.meta[r] = make_int2(part.first, count);
-    for (int i = tid; i < hn * HD; i += 256) {
+    if (tid == 0 && blockIdx.y == 0 && a.columns) {
+        if (b0 == 0) a.meta[r].x = blockIdx.x;
+        if (b1 == nb) a.meta[r].y = blockIdx.x;
+    }
+    for (int i = tid; i < hn * HD; i += 64 * pkv::kWaves) {
         const int h = i / HD, d = i % HD;
         float R = kLowest, L = 0.0f, o = 0.0f;
 #pragma unroll
@@ -553,32 +682,38 @@ __global__ __launch_bounds__(256, 2) void pkv_attend_kernel(Layer c, Attend a) {
             L = fmaf(wml[k][h].y, f, L);
             o = fmaf(wsum[k][h][d], f, o);
         }
-        if (count == 1) {
+        if (whole) {
             a.out[r * a.ldo + (int64_t)(h0 + h) * HD + d] = L == 0.0f ? 0.0f : o / L;
         } else {
-            const int64_t at = (int64_t)blockIdx.x * a.n_head + h0 + h;
-            a.sums[at * HD + d] = o;
-            if (d == 0) a.ml[at] = make_float2(R, L);
+            const int64_t slot = (int64_t)blockIdx.x * a.n_head + h0 + h;
+            a.sums[slot * HD + d] = o;
+            if (d == 0) a.ml[slot] = make_float2(R, L);
         }
     }
 }
 
-// The splits of a row put together, in their order: a workgroup a (head, row).
+// The segments of a row put together, in their order: a workgroup a (head, row).
+constexpr int kJoinWaves = 4;
 template <int HD>
-__global__ __launch_bounds__(256) void pkv_join_kernel(Attend a) {
-    __shared__ float wl[pkv::kWaves], ws[pkv::kWaves][HD];
+__global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Attend a) {
+    __shared__ float wl[kJoinWaves], ws[kJoinWaves][HD];
     const int64_t r = blockIdx.y;
     const int h = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int2 m = a.meta[r];
-    if (m.y <= 1) return;
+    int2 m = a.meta[r];
+    if (row_len(c, a, r) == 0) {  // in no slot
+        if (threadIdx.x < HD) a.out[r * a.ldo + (int64_t)h * HD + threadIdx.x] = 0.0f;
+        return;
+    }
+    if (m.x == m.y) return;  // in one, which has written it
     const float2 *ml = a.ml + (int64_t)m.x * a.n_head + h;
     const float *sums = a.sums + ((int64_t)m.x * a.n_head + h) * HD;
+    m.y = m.y - m.x + 1;
     float R = kLowest;
     for (int i = lane; i < m.y; i += 64) R = fmaxf(R, ml[(int64_t)i * a.n_head].x);
     R = llmq_wave_max_all(R);
     float L = 0.0f, o[HD / 64] = {};
 #pragma unroll 4
-    for (int i = w; i < m.y; i += pkv::kWaves) {
+    for (int i = w; i < m.y; i += kJoinWaves) {
         const float2 x = ml[(int64_t)i * a.n_head];
         const float f = exp2f(x.x - R);
         L = fmaf(x.y, f, L);
@@ -664,20 +799,23 @@ int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, Atten
     LLMQ_REQUIRE((int64_t)kv->n_kv * p.tiles <= 65535, "%s: %d query heads", name, a.n_head);
     a.rows = (int)rows;
     a.tiles = p.tiles;
-    a.shift = p.shift;
     a.meta = static_cast<int2 *>(work);
     a.ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(work) + at.ml);
     a.sums = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + at.sums);
-    // tables too short for a second split need no joining
-    const bool join = p.shift >= 0 && width * kv->page > (int64_t)pkv::kMinBlocks * pkv::block_positions(kv->elem());
-    // columns a multiple of the 8 XCDs: the tiles of one cached head land on one
-    const int64_t cols = p.shift >= 0 ? ((join ? p.slots : rows) + 7) / 8 * 8 : rows;
+    // rows that one column would take whole need no joining
+    const bool join = p.columns && width * kv->page > (int64_t)pkv::kMinBlocks * B;
+    a.columns = join ? p.columns : 0;
+    // a multiple of the 8 XCDs: the tiles of one cached head land on one
+    const int64_t cols = join ? (pkv::slots_of(p, rows) + 7) / 8 * 8 : rows;
+    LLMQ_REQUIRE(!join || rows * width * (kv->page / B) < pkv::kMaxBlocks, "%s: %lld table rows of %lld pages", name,
+                 (long long)rows, (long long)width);
     return dispatch(kv, [&](auto hd, auto elem) -> int {
         hipLaunchKernelGGL((pkv_attend_kernel<decltype(hd)::value, decltype(elem)::value>),
-                           dim3((unsigned)cols, (unsigned)(kv->n_kv * p.tiles)), dim3(256), 0, ctx->stream, c, a);
+                           dim3((unsigned)cols, (unsigned)(kv->n_kv * p.tiles)), dim3(64 * pkv::kWaves), 0, ctx->stream,
+                           c, a);
         if (join)
             hipLaunchKernelGGL((pkv_join_kernel<decltype(hd)::value>), dim3((unsigned)a.n_head, (unsigned)rows),
-                               dim3(256), 0, ctx->stream, a);
+                               dim3(64 * kJoinWaves), 0, ctx->stream, c, a);
         LLMQ_HIP(hipGetLastError());
         return LLMQ_OK;
     });
@@ -717,8 +855,9 @@ int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int p
         llmq_pkv_free(kv);
         return llmq_set_error(LLMQ_ENOMEM, "pkv_create: allocation of %zu bytes failed", 2 * n + (scales ? 2 * ns : 0));
     }
-    if (hipMemsetAsync(kv->k, 0, n, ctx->stream) != hipSuccess ||
-        hipMemsetAsync(kv->v, 0, n, ctx->stream) != hipSuccess ||
+    const int zero = scales ? kBias : 0;  // the code of 0
+    if (hipMemsetAsync(kv->k, zero, n, ctx->stream) != hipSuccess ||
+        hipMemsetAsync(kv->v, zero, n, ctx->stream) != hipSuccess ||
         (scales && (hipMemsetAsync(kv->ks, 0, ns, ctx->stream) != hipSuccess ||
                     hipMemsetAsync(kv->vs, 0, ns, ctx->stream) != hipSuccess))) {
         llmq_pkv_free(kv);

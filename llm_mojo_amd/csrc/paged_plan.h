@@ -12,20 +12,15 @@
 
 namespace pkv {
 
-// A cache element is an int8 code or a float16 value (2 bytes).  A block is
-// the positions a wave of the attention takes at a time: NT tiles of 16, so
-// that one position's 16 * NT / 4 elements of a lane fill 16 bytes.
-PKV_HD int block_positions(int elem) { return elem == 1 ? 64 : 32; }
+// A block is the positions a wave of the attention takes at a time: two
+// tiles of 16.
+constexpr int kBlock = 32;
 
 // Values are kept transposed a block, [block][dimension][slot]: position p =
-// 16 t + 4 q + i of its block (t < NT, q < 4, i < 4) in slot (q NT + t) 4 + i,
-// so the 4 NT positions that matrix-core lanes of quarter q multiply are 16
-// consecutive bytes.
-PKV_HD int value_slot(int elem, int p) {
-    const int nt = elem == 1 ? 4 : 2;
-    const int t = p >> 4, q = (p >> 2) & 3, i = p & 3;
-    return (q * nt + t) * 4 + i;
-}
+// 16 t + 4 q + i of its block (t < 2, q < 4, i < 4) in slot 8 q + 4 t + i, so
+// the eight positions that matrix-core lanes of quarter q multiply lie
+// together.
+PKV_HD int value_slot(int p) { return ((p >> 2) & 3) * 8 + (p >> 4) * 4 + (p & 3); }
 
 // The page of position `pos` of a table row of `width` pages, or -1 where
 // the position or the page is none of the cache's (`pages` of `page`
@@ -43,48 +38,50 @@ PKV_HD int64_t clamp_len(int64_t len, int64_t width, int page) {
 }
 
 // How a call's rows are split over workgroups.  A workgroup takes up to 8 of
-// the query heads of a cached head (`tiles` of them cover the group).  Up to kPlanRows rows,
-// the blocks of all rows are dealt into splits of one size, the least that
-// leaves at most 2^shift splits' worth of whole ones (and kMinBlocks, a
-// block a wave): a long row gets many, a short one one, and there are never
-// more than `slots`.  More rows fill the card by themselves and are not split (shift -1).
-constexpr int kWaves = 4;        // of a workgroup, each taking every kWaves-th block
-constexpr int kMinBlocks = 4;    // blocks of the smallest split
-constexpr int kPlanRows = 256;   // rows whose lengths a wave holds at once
-constexpr int kWorkgroups = 1024;  // aimed at, over all heads
+// the query heads of a cached head (`tiles` of them cover the group).  Up to
+// kPlanRows rows, the blocks of all rows in one line are cut into columns of
+// one size, and a workgroup takes what a column has of a row (a segment): a
+// long row gets many, a short one one.  More rows fill the card by
+// themselves: a workgroup a row (columns 0).
+constexpr int kWaves = 4;         // of a workgroup, each taking every kWaves-th block
+constexpr int kMinBlocks = 16;    // of a column
+constexpr int kPlanRows = 256;    // rows whose lengths a wave holds at once
+constexpr int kWorkgroups = 2048;
+constexpr int64_t kMaxBlocks = (int64_t)1 << 31;  // of all rows' tables, where they are cut into columns
 
 struct Plan {
-    int tiles, shift;
-    int64_t slots;
+    int tiles, columns;
 };
 
 PKV_HD Plan plan_of(int64_t rows, int n_head, int n_kv) {
     Plan p;
     p.tiles = (n_head / n_kv + 7) / 8;
-    p.shift = -1;
-    p.slots = rows;
+    p.columns = 0;
     if (rows > kPlanRows) return p;
-    p.shift = 0;
-    while (((int64_t)n_kv * p.tiles << (p.shift + 1)) <= kWorkgroups) p.shift++;
-    p.slots = rows + ((int64_t)1 << p.shift);
+    const int64_t all = (int64_t)n_kv * p.tiles;
+    p.columns = all >= kWorkgroups ? 1 : (int)(kWorkgroups / all);
     return p;
 }
 
-// Blocks a split, given those of all rows; and splits of a row of nb blocks (at least one, for the row's output).
-PKV_HD int64_t split_blocks(int64_t total, int shift) {
-    const int64_t n = (total >> shift) + 1;
-    return n < kMinBlocks ? kMinBlocks : (n > 0x7fffffff ? 0x7fffffff : n);
+// Blocks of a column, given those of all rows: at most `columns` columns, a multiple of the waves.
+PKV_HD uint32_t column_blocks(uint32_t total, int columns) {
+    const uint32_t n = total / (uint32_t)columns + 1;
+    return n < (uint32_t)kMinBlocks ? (uint32_t)kMinBlocks : (n + kWaves - 1) / kWaves * kWaves;
 }
-PKV_HD uint32_t row_splits(uint32_t nb, uint32_t blocks) { return nb <= blocks ? 1 : (nb - 1) / blocks + 1; }
 
-// Byte offsets of a call's workspace: per row the first split and their
-// number, per (split, head) the reference and sum of its exponentials, and its sums of values.
+// Row r, whose blocks are [begin, end) of the line, has its segments of columns begin / per ... in slots
+// r + column: the pairs of (row, column) go up in one or both along the line, so no two share a slot, and
+// the row of a slot is the number of rows k with k + 1 + end of k / per at most the slot.
+PKV_HD int64_t slots_of(const Plan &p, int64_t rows) { return p.columns ? p.columns + rows : 0; }
+
+// Byte offsets of a call's workspace: per row its first and last column, per
+// (slot, head) the reference and sum of its exponentials, and its sums of values.
 struct Work {
     int64_t ml, sums, bytes;
 };
 PKV_HD Work work_of(const Plan &p, int64_t rows, int n_head, int hd) {
     Work w;
-    const int64_t slots = p.shift < 0 ? 0 : p.slots;
+    const int64_t slots = slots_of(p, rows);
     w.ml = (rows * 8 + 255) & ~(int64_t)255;
     w.sums = w.ml + ((slots * n_head * 8 + 255) & ~(int64_t)255);
     w.bytes = w.sums + slots * n_head * hd * 4;

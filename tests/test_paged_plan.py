@@ -13,18 +13,16 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SRC = """
 #include "paged_plan.h"
 extern "C" {
-int block_positions(int e) { return pkv::block_positions(e); }
-int value_slot(int e, int p) { return pkv::value_slot(e, p); }
+int value_slot(int p) { return pkv::value_slot(p); }
 int page_of(const int32_t *row, int64_t w, int page, int64_t pages, int64_t pos) {
     return pkv::page_of(row, w, page, pages, pos); }
 int64_t clamp_len(int64_t n, int64_t w, int page) { return pkv::clamp_len(n, w, page); }
 void plan(int64_t rows, int n_head, int n_kv, int hd, int64_t *out) {
     const pkv::Plan p = pkv::plan_of(rows, n_head, n_kv);
     const pkv::Work w = pkv::work_of(p, rows, n_head, hd);
-    out[0] = p.tiles; out[1] = p.shift; out[2] = p.slots; out[3] = w.ml; out[4] = w.sums; out[5] = w.bytes;
+    out[0] = p.tiles; out[1] = p.columns; out[2] = pkv::slots_of(p, rows); out[3] = w.ml; out[4] = w.sums; out[5] = w.bytes;
 }
-int64_t split_blocks(int64_t total, int shift) { return pkv::split_blocks(total, shift); }
-uint32_t row_splits(uint32_t nb, uint32_t blocks) { return pkv::row_splits(nb, blocks); }
+uint32_t column_blocks(uint32_t total, int columns) { return pkv::column_blocks(total, columns); }
 }
 """
 
@@ -40,22 +38,16 @@ def plan(tmp_path_factory):
     i64 = ctypes.c_int64
     L.page_of.argtypes = [ctypes.c_void_p, i64, ctypes.c_int, i64, i64]
     L.plan.argtypes = [i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
-    L.split_blocks.argtypes, L.split_blocks.restype = [i64, ctypes.c_int], i64
-    L.row_splits.argtypes, L.row_splits.restype = [ctypes.c_uint32] * 2, ctypes.c_uint32
+    L.column_blocks.argtypes, L.column_blocks.restype = [ctypes.c_uint32, ctypes.c_int], ctypes.c_uint32
     L.clamp_len.argtypes, L.clamp_len.restype = [i64, i64, ctypes.c_int], i64
     return L
 
 
-@pytest.mark.parametrize("elem", [1, 2])
-def test_value_slots(plan, elem):
-    b = plan.block_positions(elem)
-    nt = b // 16
-    assert b * elem == 64
-    slots = [plan.value_slot(elem, p) for p in range(b)]
-    assert sorted(slots) == list(range(b))
-    for q in range(4):  # quarter q's bytes: its positions of tile 0, 1, ..
-        mine = [slots.index(s) for s in range(q * 4 * nt, (q + 1) * 4 * nt)]
-        assert mine == [16 * t + 4 * q + i for t in range(nt) for i in range(4)]
+def test_value_slots(plan):
+    slots = [plan.value_slot(p) for p in range(32)]
+    assert sorted(slots) == list(range(32))
+    for q in range(4):  # quarter q's: its positions of tile 0, then of tile 1
+        assert [slots.index(s) for s in range(8 * q, 8 * q + 8)] == [16 * t + 4 * q + i for t in (0, 1) for i in range(4)]
 
 
 def test_pages_stay_inside(plan):
@@ -83,35 +75,43 @@ def blocks(rng, rows):
     kind = rng.integers(0, 4)
     if kind == 0:
         return np.zeros(rows, np.int64)
-    nb = (2.0 ** rng.uniform(0, (6, 12, 26)[kind - 1], rows)).astype(np.int64)
+    nb = (2.0 ** rng.uniform(0, (6, 12, 22)[kind - 1], rows)).astype(np.int64)
     nb[rng.random(rows) < 0.2] = 0
     if kind == 3:
-        nb[rng.integers(0, rows)] = 2 ** 26 - 1
+        nb[rng.integers(0, rows)] = 2 ** 31 - 1 - nb.sum()
     return nb
 
 
-def test_splits_cover_the_rows_and_fit(plan):
-    """Any lengths: every block of every row is in one split, each row has at
-    least one, and there are no more splits than the grid and the workspace
-    hold."""
+def test_columns_cover_the_rows_and_fit(plan):
+    """Any lengths: every block is in one slot's segment, found from the slot
+    as the kernel does, and the slots fit the grid and the workspace."""
     rng = np.random.default_rng(1)
     out = np.zeros(6, np.int64)
-    for _ in range(4000):
+    for _ in range(1500):
         rows = int(2 ** rng.uniform(0, 8))
-        n_kv = int(rng.choice([1, 2, 3, 4, 8, 12, 32, 129]))
+        n_kv = int(rng.choice([1, 2, 3, 4, 8, 12, 32, 129, 600, 2000]))
         n_head = n_kv * int(rng.choice([1, 2, 7, 8, 9, 16, 71]))
         hd = int(rng.choice([64, 128]))
         plan.plan(rows, n_head, n_kv, hd, out.ctypes.data)
-        tiles, shift, slots, ml, sums, size = (int(x) for x in out)
+        tiles, columns, slots, ml, sums, size = (int(x) for x in out)
         assert tiles * 8 >= n_head // n_kv > (tiles - 1) * 8
-        assert shift >= 0 and (shift == 0 or (n_kv * tiles << shift) <= 1024) and slots == rows + 2 ** shift
+        assert columns >= 1 and (columns == 1 or n_kv * tiles * columns <= 2048) and slots == rows + columns
         assert ml >= rows * 8 and sums >= ml + slots * n_head * 8 and size == sums + slots * n_head * hd * 4
         assert ml % 256 == 0 and sums % 256 == 0
         nb = blocks(rng, rows)
-        per = plan.split_blocks(int(nb.sum()), shift)
-        assert 4 <= per <= 2 ** 31 - 1
-        n = np.array([plan.row_splits(int(x), per) for x in nb])
-        assert (n >= 1).all() and (n * per >= nb).all() and ((n - 1) * per < np.maximum(nb, 1)).all()
-        assert n.sum() <= slots
+        total = int(nb.sum())
+        per = plan.column_blocks(total, columns)
+        assert per >= 16 and per % 4 == 0 and -(-total // per) <= columns and per <= 2 ** 31
+        ends = np.cumsum(nb)
+        covered = np.zeros(rows, np.int64)
+        for s in range(slots):
+            r = int((np.arange(rows) + 1 + ends // per <= s).sum())
+            j = s - r
+            if r >= rows or j < 0:
+                continue
+            lo, hi = max(j * per, ends[r] - nb[r]), min((j + 1) * per, ends[r])
+            if lo < hi:
+                covered[r] += hi - lo
+        assert (covered == nb).all()
     plan.plan(257, 12, 12, 64, out.ctypes.data)
-    assert out[1] == -1 and out[2] == 257 and out[5] == out[4]
+    assert out[1] == 0 and out[2] == 0 and out[5] == out[4]
