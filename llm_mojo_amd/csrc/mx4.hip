@@ -12,7 +12,8 @@
 // Device layout of a matrix: rows in tiles of 16, codes [tile][step][lane][16
 // bytes] (a wave's operand is 1 KB in one piece), scales [tile][step /
 // 4][lane][4 bytes] (four steps' bytes a word, the instruction selects one).
-// Rows and blocks past the matrix's end are zero codes with scale 127.
+// A tile has whole words of four steps; rows and blocks past the matrix's end
+// are zero codes with scale 127.
 #include <math.h>
 
 #include <new>
@@ -73,35 +74,99 @@ __device__ __forceinline__ float code_value(int c) {
     return c & 8 ? -v : v;
 }
 
-// llmq_mx4_quantize: a thread a block.
-__global__ __launch_bounds__(256) void mx4_quantize_kernel(const float *__restrict__ x, int64_t ldx, int64_t nb,
-                                                           int64_t total, uint4 *__restrict__ codes,
-                                                           uint8_t *__restrict__ scales) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const float *p = x + (i / nb) * ldx + (i % nb) * 32;
-    float v[32];
-#pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = p[j];
-    int e;
-    codes[i] = quant_block(v, &e);
-    scales[i] = (uint8_t)e;
+struct Float4 {
+    float x[4];
+} __attribute__((packed, aligned(4)));
+
+// Largest magnitude over the four lanes of a block (quad permutes); NaN counts as above all.
+__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));
+    return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));
 }
 
-__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t *__restrict__ codes,
-                                                             const uint8_t *__restrict__ scales, int64_t nb,
+// The scale byte of a block whose largest magnitude has these bits.
+__device__ __forceinline__ int scale_of_bits(uint32_t m) {
+    const int e = (int)(m >> 23) - 2;
+    return m >= 0x7f800000u ? 255 : (e < 0 ? 0 : e);
+}
+
+// One lane's quarter of a block: its 8 codes, and the block's scale byte.
+__device__ __forceinline__ uint32_t quant_quarter(const float (&x)[8], int *scale) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    const int e = scale_of_bits(quad_max(m));
+    *scale = e;
+    return e == 255 ? 0u : codes8(x, inverse_scale(e));
+}
+
+// llmq_mx4_quantize: a lane 8 values, four lanes a block, kQuant blocks'
+// quarters a lane.  Bound by reading the floats; unit = K / 8 lanes a row
+// (one row of them all where the rows lie together).
+constexpr int kQuant = 4;
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const float *__restrict__ x, int64_t ldx, uint32_t unit,
+                                                           int64_t total, uint32_t *__restrict__ codes,
+                                                           uint8_t *__restrict__ scales) {
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * kQuant) + threadIdx.x;
+    float v[kQuant][8];
+#pragma unroll
+    for (int k = 0; k < kQuant; k++) {
+        const int64_t i = i0 + 256 * k;
+        if (i < total) {  // the four lanes of a block are in or out together
+            const float *p = x + (unit ? (i / unit) * ldx + (i % unit) * 8 : i * 8);
+            const Float4 a = *reinterpret_cast<const Float4 *>(p), b = *reinterpret_cast<const Float4 *>(p + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[k][j] = a.x[j];
+                v[k][4 + j] = b.x[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kQuant; k++) {
+        const int64_t i = i0 + 256 * k;
+        if (i < total) {
+            int e;
+            codes[i] = quant_quarter(v[k], &e);
+            if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)e;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t *__restrict__ codes,
+                                                             const uint8_t *__restrict__ scales, uint32_t unit,
                                                              int64_t total, float *__restrict__ out, int64_t ldo) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    float *p = out + (i / nb) * ldo + (i % nb) * 32;
-    const float s = scale_value(scales[i]);
-    for (int j = 0; j < 32; j++) p[j] = code_value((codes[i * 16 + j / 2] >> (4 * (j & 1))) & 15) * s;
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * kQuant) + threadIdx.x;
+    uint32_t c[kQuant];
+    float s[kQuant];
+#pragma unroll
+    for (int k = 0; k < kQuant; k++) {
+        const int64_t i = i0 + 256 * k;
+        if (i < total) {
+            c[k] = codes[i];
+            s[k] = scale_value(scales[i >> 2]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kQuant; k++) {
+        const int64_t i = i0 + 256 * k;
+        if (i >= total) continue;
+        float *p = out + (unit ? (i / unit) * ldo + (i % unit) * 8 : i * 8);
+        Float4 a, b;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            a.x[j] = code_value((c[k] >> (4 * j)) & 15) * s[k];
+            b.x[j] = code_value((c[k] >> (4 * j + 16)) & 15) * s[k];
+        }
+        *reinterpret_cast<Float4 *>(p) = a;
+        *reinterpret_cast<Float4 *>(p + 4) = b;
+    }
 }
 
 // A weight matrix from floats: a thread a (row, block); with reduce_rows
 // (source [IN, OUT]) neighbouring threads read neighbouring floats.
 __global__ __launch_bounds__(256) void mx4_weights_kernel(const float *__restrict__ src, int64_t cols, int reduce_rows,
-                                                          int64_t n, int64_t nb, int64_t steps, int64_t words,
+                                                          int64_t n, int64_t nb, int64_t words,
                                                           uint4 *__restrict__ codes, uint8_t *__restrict__ scales) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n * nb) return;
@@ -113,7 +178,7 @@ __global__ __launch_bounds__(256) void mx4_weights_kernel(const float *__restric
     const uint4 c = quant_block(v, &e);
     const int64_t tile = o >> 4, step = b >> 2;
     const int lane = (int)(o & 15) + 16 * (int)(b & 3);
-    codes[(tile * steps + step) * 64 + lane] = c;
+    codes[(tile * words * 4 + step) * 64 + lane] = c;
     scales[((tile * words + (step >> 2)) * 64 + lane) * 4 + (step & 3)] = (uint8_t)e;
 }
 
@@ -125,38 +190,294 @@ __device__ __forceinline__ void finish(float *p, float y, const float *bias, int
     *p = y;
 }
 
-// One wave a (16 outputs, 16 tokens).
-__global__ __launch_bounds__(64) void mx4_linear_kernel(const uint4 *__restrict__ xc, const uint8_t *__restrict__ xs,
-                                                        const uint4 *__restrict__ wc, const uint32_t *__restrict__ ws,
-                                                        int64_t T, int64_t n, int64_t nb, int64_t steps, int64_t words,
-                                                        float *__restrict__ out, const float *__restrict__ bias,
-                                                        int flags) {
-    const int lane = threadIdx.x, q = lane >> 4;
-    const int64_t tile = blockIdx.x, t = (int64_t)blockIdx.y * 16 + (lane & 15);
-    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t s = 0; s < steps; s++) {
-        const uint4 a = wc[(tile * steps + s) * 64 + lane];
-        const int as = (int)(ws[(tile * words + (s >> 2)) * 64 + lane] >> (8 * (s & 3)));
-        const int64_t b = s * 4 + q;
-        const bool in = t < T && b < nb;
-        const uint4 x = in ? xc[t * nb + b] : make_uint4(0, 0, 0, 0);
-        const int bs = in ? xs[t * nb + b] : 127;
-        const v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0},
-                  bv = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0};
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, as, 0, bs);
+// Operands of a product: tokens quantized in rows (codes K / 2 and scales
+// K / 32 bytes each; nb blocks), the matrix in its layout.
+struct Product {
+    const uint8_t *xc, *xs;
+    const uint8_t *wc;
+    const uint32_t *ws;
+    const float *x;  // one token's floats instead of xc, xs
+    int64_t T;
+    int n, nb, steps, words, ntiles;
+    float *out;
+    const float *bias;
+    int flags;
+};
+
+__device__ __forceinline__ v4f mma(const uint4 &a, const uint4 &b, const v4f &c, int as, int bs, int sel) {
+    const v8i x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0},
+              y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    switch (sel) {  // a constant after unrolling
+        case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, as, 0, bs);
+        case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 1, as, 1, bs);
+        case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 2, as, 2, bs);
+        default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 3, as, 3, bs);
     }
-    if (t >= T) return;
-    for (int i = 0; i < 4; i++) {
-        const int64_t o = tile * 16 + 4 * q + i;
-        if (o < n) finish(out + t * n + o, acc[i], bias, o, flags);
+}
+
+// The scale bytes of blocks q, 4 + q, 8 + q, 12 + q of a token's 16 blocks
+// from block 16 g, in one word (a step a byte).  Blocks past the row's end
+// get 127: their weights are zeros, which a NaN there would spoil.
+struct Bytes16 {
+    uint32_t x[4];
+} __attribute__((packed, aligned(1)));
+__device__ __forceinline__ uint32_t token_scales(const uint8_t *row, int nb, int g, int q) {
+    if (g * 16 + 16 <= nb) {
+        const Bytes16 s = *reinterpret_cast<const Bytes16 *>(row + g * 16);
+        const uint32_t sel = 0x0400u + 0x0101u * q;
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(s.x[3], s.x[2], sel),
+                                     __builtin_amdgcn_perm(s.x[1], s.x[0], sel), 0x05040100u);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int b = g * 16 + 4 * j + q;
+        w |= (b < nb ? (uint32_t)row[b] : 127u) << (8 * j);
+    }
+    return w;
+}
+
+// Waves of a few-token workgroup at most: with four token tiles its registers hold half as many.
+constexpr int few_most(int tt) { return tt < 4 ? 16 : 8; }
+
+// Few tokens: a workgroup 16 outputs and TT tiles of 16 tokens, its waves
+// taking whole groups of four steps in turn (`per` each), their sums added in
+// LDS in wave order.  Bound by the weights, read once a TT tiles; all of a
+// group's operands are asked for before the first product.  FUSED: one token
+// from its floats, quantized by every workgroup into LDS while its weights
+// are on their way, in place of a launch that writes 17 / 32 K bytes.
+template <int TT, bool FUSED>
+__global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, int per) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4,
+              c = lane & 15, waves = blockDim.x >> 6;
+    const int tile = blockIdx.x;
+    const int64_t t0 = (int64_t)blockIdx.y * (16 * TT);
+    const auto rw = llmq_rsrc(p.wc + (int64_t)tile * p.words * 4096, (uint32_t)p.steps * 1024);
+    const uint32_t *ws = p.ws + (int64_t)tile * p.words * 64 + lane;
+    const int rowb = p.nb * 16;
+    const int64_t left = p.T - t0;
+    const int live = (int)(left < 16 * TT ? left : 16 * TT);
+    const auto rx = llmq_rsrc(FUSED ? p.wc : p.xc + t0 * rowb, FUSED ? 0 : (uint32_t)live * rowb);
+    uint8_t *fs = lds, *fc = lds + p.words * 16;  // FUSED: scales [group][q][step], codes
+
+    uint4 a[4];
+    uint32_t as = 0;
+    auto weights = [&](int g) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)  // zeros past the last step, without reading them
+            a[j] = llmq_bload16(rw, lane * 16 + (g * 4 + j) * 1024);
+        as = ws[g * 64];
+    };
+    int g = w * per;
+    const int end = min(g + per, p.words);
+    if (g < end) weights(g);
+    if constexpr (FUSED) {
+        const int units = p.words * 64;  // quarters of blocks
+        for (int i = tid; i < units; i += blockDim.x) {
+            float v[8];
+            int e = 127;
+            uint32_t code = 0;
+            if (i < p.nb * 4) {
+                const Float4 x = *reinterpret_cast<const Float4 *>(p.x + i * 8),
+                             y = *reinterpret_cast<const Float4 *>(p.x + i * 8 + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    v[j] = x.x[j];
+                    v[4 + j] = y.x[j];
+                }
+                code = quant_quarter(v, &e);
+            }
+            reinterpret_cast<uint32_t *>(fc)[i] = code;
+            const int blk = i >> 2;
+            if ((i & 3) == 0) fs[(blk & ~15) + (blk & 3) * 4 + ((blk >> 2) & 3)] = (uint8_t)e;
+        }
+        __syncthreads();
+    }
+    v4f acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; t++) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (; g < end; g++) {
+        uint4 b[TT][4];
+        uint32_t bs[TT];
+#pragma unroll
+        for (int t = 0; t < TT; t++) {
+            if constexpr (FUSED) {  // the token in every column
+                bs[t] = *reinterpret_cast<const uint32_t *>(fs + g * 16 + q * 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) b[t][j] = *reinterpret_cast<const uint4 *>(fc + (g * 4 + j) * 64 + q * 16);
+            } else {
+                const int row = min(16 * t + c, live - 1);
+                bs[t] = token_scales(p.xs + (t0 + row) * p.nb, p.nb, g, q);
+#pragma unroll
+                for (int j = 0; j < 4; j++) b[t][j] = llmq_bload16(rx, row * rowb + q * 16 + (g * 4 + j) * 64);
+            }
+        }
+        uint4 u[4];
+        const uint32_t us = as;
+#pragma unroll
+        for (int j = 0; j < 4; j++) u[j] = a[j];
+        if (g + 1 < end) weights(g + 1);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int t = 0; t < TT; t++) acc[t] = mma(u[j], b[t][j], acc[t], (int)us, (int)bs[t], j);
+    }
+    // [wave][tile][token][output]
+    float *sum = reinterpret_cast<float *>(lds);
+    if constexpr (FUSED) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+        if (!FUSED || c == 0)
+            *reinterpret_cast<v4f *>(sum + ((w * TT + t) * 16 + c) * 16 + 4 * q) = acc[t];
+    __syncthreads();
+    for (int i = tid; i < live * 16; i += blockDim.x) {
+        const int o = tile * 16 + (i & 15);
+        float y = sum[i];
+        for (int k = 1; k < waves; k++) y += sum[k * TT * 256 + i];
+        if (o < p.n) finish(p.out + (t0 + (i >> 4)) * p.n + o, y, p.bias, o, p.flags);
+    }
+}
+
+// Many tokens: a workgroup 256 outputs and 128 tokens, a wave 64 of the
+// outputs by all the tokens (32 accumulators).  The tokens' codes are shared
+// by the four waves: they are copied to LDS a group of four steps ahead, each
+// fragment as the 1 KB that a wave reads of it, without passing through
+// registers; their scales are put into words there a group ahead.  A wave's
+// weights, which no other wave of the workgroup reads, come straight to its
+// registers two steps ahead, 1 KB in one piece.  A step is 32 products of 16
+// cycles to 8 KB of LDS reads a wave: half of what LDS gives.
+constexpr int kTokens = 128, kOuts = 256;
+__global__ __launch_bounds__(256, 2) void mx4_many_kernel(Product p, int gx, int gy) {
+    __shared__ __align__(16) uint8_t c0[32768], c1[32768];
+    __shared__ uint32_t s0[512], s1[512];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4,
+              c = lane & 15;
+    // an XCD takes neighbouring tiles, the tokens' fastest: it reads its part of the weights once
+    const int all = gx * gy, xcd = blockIdx.x & 7, at = blockIdx.x >> 3, each = all >> 3, more = all & 7;
+    const int pos = xcd * each + min(xcd, more) + at;
+    const int bo = pos / gy, bt = pos % gy;
+    const int64_t t0 = (int64_t)bt * kTokens;
+    const int rowb = p.nb * 16;
+    const int64_t left = p.T - t0;
+    const int live = (int)(left < kTokens ? left : kTokens);
+    const auto rx = llmq_rsrc(p.xc + t0 * rowb, (uint32_t)live * rowb);
+    const int tile0 = bo * 16 + w * 4;
+    int so[4];  // the wave's row tiles (its first again past the matrix's end)
+    const int base = min(tile0, p.ntiles - 1);
+#pragma unroll
+    for (int r = 0; r < 4; r++) so[r] = (min(tile0 + r, p.ntiles - 1) - base);
+    const auto rw = llmq_rsrc(p.wc + (int64_t)base * p.words * 4096,
+                              (uint32_t)min(4, p.ntiles - base) * (uint32_t)p.words * 4096);
+    const uint32_t *ws = p.ws + (int64_t)base * p.words * 64 + lane;
+    const int groups = p.words;
+
+    auto stage = [&](int g, uint8_t *dst) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int t = 2 * w + i;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rx, (__attribute__((address_space(3))) void *)(dst + (j * 8 + t) * 1024), 16,
+                    (16 * t + c) * rowb + q * 16 + (g * 4 + j) * 64, 0, 0, 0);
+            }
+    };
+    auto scales = [&](int g, uint32_t *dst) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = tid + 256 * k, row = min(i >> 6 << 4 | (i & 15), live - 1);
+            dst[i] = token_scales(p.xs + (t0 + row) * p.nb, p.nb, g, (i >> 4) & 3);
+        }
+    };
+    v4f acc[4][8];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int t = 0; t < 8; t++) acc[r][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    uint4 a[3][4];
+    auto weights = [&](int s, uint4 (&dst)[4]) __attribute__((always_inline)) {
+        const int k = min(s, 4 * p.words - 1);  // (past the end: loaded and not used)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(rw, lane * 16, (so[r] * 4 * p.words + k) * 1024, 0);
+            dst[r] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    };
+    uint32_t as[4], an[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) as[r] = ws[so[r] * p.words * 64];
+    stage(0, c0);
+    scales(0, s0);
+    weights(0, a[0]);
+    weights(1, a[1]);
+    auto group = [&](int g, const uint8_t *cb, uint8_t *nb, const uint32_t *sb, uint32_t *ns)
+        __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this wave's copies are in, its reads done
+        llmq_lds_barrier();
+        const bool next = g + 1 < groups;
+        if (next) {
+            stage(g + 1, nb);
+#pragma unroll
+            for (int r = 0; r < 4; r++) an[r] = ws[(so[r] * p.words + g + 1) * 64];
+        }
+        uint32_t bs[8];
+#pragma unroll
+        for (int t = 0; t < 8; t++) bs[t] = sb[t * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int s = g * 4 + j;
+            weights(s + 2, a[(j + 2) % 3]);
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                const uint4 b = *reinterpret_cast<const uint4 *>(cb + (j * 8 + t) * 1024 + lane * 16);
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[r][t] = mma(a[j % 3][r], b, acc[r][t], (int)as[r], (int)bs[t], j);
+            }
+        }
+        // four steps on, the ring of three has moved by one
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint4 x = a[1][r], y = a[2][r];
+            a[0][r] = x;
+            a[1][r] = y;
+            as[r] = an[r];
+        }
+        if (next) scales(g + 1, ns);
+    };
+    for (int g = 0; g < groups; g += 2) {
+        group(g, c0, c1, s0, s1);
+        if (g + 1 < groups) group(g + 1, c1, c0, s1, s0);
+    }
+    const bool wide = p.n % 4 == 0 && (uintptr_t)p.out % 16 == 0 && !(p.flags & ~LLMQ_BIAS);
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+        if (16 * t + c >= live) continue;
+        float *row = p.out + (t0 + 16 * t + c) * p.n;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int o = (tile0 + r) * 16 + 4 * q;
+            if (wide) {
+                if (o >= p.n) continue;
+                v4f y = acc[r][t];
+                if (p.flags & LLMQ_BIAS)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[i] += p.bias[o + i];
+                *reinterpret_cast<v4f *>(row + o) = y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (o + i < p.n) finish(row + o + i, acc[r][t][i], p.bias, o + i, p.flags);
+            }
+        }
     }
 }
 
 int check_shape(const char *name, int64_t rows, int64_t cols) {
     LLMQ_REQUIRE(rows > 0 && cols > 0, "%s: empty matrix", name);
     LLMQ_REQUIRE(cols % 32 == 0, "%s: %lld inputs are no whole blocks of 32", name, (long long)cols);
-    LLMQ_REQUIRE(rows <= INT32_MAX - 64 && cols <= INT32_MAX - 1024, "%s: %lld x %lld matrix", name, (long long)rows,
-                 (long long)cols);
+    LLMQ_REQUIRE(rows <= INT32_MAX - 512 && cols <= 1 << 24, "%s: %lld x %lld matrix (at most 2^24 inputs)", name,
+                 (long long)rows, (long long)cols);
     return LLMQ_OK;
 }
 
@@ -172,7 +493,7 @@ int mx4_alloc(llmq_ctx *ctx, int64_t n, int64_t k, llmq_mat **out) {
     m->ntiles = (n + 15) / 16;
     m->CK = (k + 127) / 128;
     m->NG = (m->CK + 3) / 4;
-    const size_t cb = (size_t)(m->ntiles * m->CK) * 1024, sb = (size_t)(m->ntiles * m->NG) * 256;
+    const size_t cb = (size_t)(m->ntiles * m->NG) * 4096, sb = (size_t)(m->ntiles * m->NG) * 256;
     if (hipMalloc(&m->codes, cb) != hipSuccess || hipMalloc(&m->scales, sb) != hipSuccess) {
         (void)hipGetLastError();
         llmq_mat_free(m);
@@ -193,38 +514,91 @@ struct Place {
 };
 Place place_of(const llmq_mat *m, int64_t o, int64_t b) {
     const int64_t tile = o >> 4, step = b >> 2, lane = (o & 15) + 16 * (b & 3);
-    return Place{(tile * m->CK + step) * 64 + lane, ((tile * m->NG + (step >> 2)) * 64 + lane) * 4 + (step & 3)};
+    return Place{(tile * m->NG * 4 + step) * 64 + lane, ((tile * m->NG + (step >> 2)) * 64 + lane) * 4 + (step & 3)};
 }
 
 int check_codes(const char *name, const llmq_ctx *ctx, const void *a, const void *codes, const void *scales, int64_t T,
                 int64_t K) {
     LLMQ_REQUIRE(ctx && ((a && codes && scales) || T == 0), "%s: null argument", name);
-    LLMQ_REQUIRE(T >= 0 && T <= INT32_MAX && K > 0 && K % 32 == 0 && K <= INT32_MAX - 1024,
+    LLMQ_REQUIRE(T >= 0 && T <= INT32_MAX && K > 0 && K % 32 == 0 && K <= 1 << 24,
                  "%s: %lld rows of %lld (whole blocks of 32)", name, (long long)T, (long long)K);
     LLMQ_REQUIRE((uintptr_t)codes % 16 == 0, "%s: codes are 16-byte aligned", name);
     return LLMQ_OK;
 }
 
+// The quarter-block kernels' grid, and lanes a row (0: the rows lie together).
+struct Quarters {
+    int64_t total, grid;
+    uint32_t unit;
+};
+int quarters(const char *name, int64_t T, int64_t K, int64_t ld, Quarters *out) {
+    out->total = T * (K / 8);
+    out->grid = (out->total + 256 * kQuant - 1) / (256 * kQuant);
+    out->unit = ld == K || T == 1 ? 0 : (uint32_t)(K / 8);
+    LLMQ_REQUIRE(out->grid <= INT32_MAX, "%s: %lld rows of %lld", name, (long long)T, (long long)K);
+    return LLMQ_OK;
+}
+
 int launch_quantize(llmq_ctx *ctx, const float *x, int64_t ldx, int64_t T, int64_t K, uint8_t *codes,
                     uint8_t *scales) {
-    const int64_t nb = K / 32, total = T * nb, grid = (total + 255) / 256;
-    LLMQ_REQUIRE(grid <= INT32_MAX, "mx4_quantize: %lld rows of %lld", (long long)T, (long long)K);
-    hipLaunchKernelGGL(mx4_quantize_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, x, ldx, nb, total,
-                       reinterpret_cast<uint4 *>(codes), scales);
+    Quarters u;
+    RC(quarters("mx4_quantize", T, K, ldx, &u));
+    hipLaunchKernelGGL(mx4_quantize_kernel, dim3((unsigned)u.grid), dim3(256), 0, ctx->stream, x, ldx, u.unit, u.total,
+                       reinterpret_cast<uint32_t *>(codes), scales);
     LLMQ_HIP(hipGetLastError());
     return LLMQ_OK;
 }
 
-int launch_product(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scales, const llmq_mat *w, int64_t T, float *out,
-                   const float *bias, int flags) {
-    const int64_t tt = (T + 15) / 16;
-    LLMQ_REQUIRE(tt <= 65535, "mx4_linear: %lld tokens", (long long)T);
-    hipLaunchKernelGGL(mx4_linear_kernel, dim3((unsigned)w->ntiles, (unsigned)tt), dim3(64), 0, ctx->stream,
-                       reinterpret_cast<const uint4 *>(codes), scales, reinterpret_cast<const uint4 *>(w->codes),
-                       reinterpret_cast<const uint32_t *>(w->scales), T, w->n, w->k / 32, w->CK, w->NG, out, bias,
-                       flags);
+// Tokens from which on the 256 x 128 kernel runs.
+constexpr int64_t kMany = 65;
+
+// Waves of a few-token workgroup, and groups of steps each: a wave a group as far as they go.
+int few_waves(const llmq_mat *w, int most, int *per) {
+    *per = (int)((w->NG + most - 1) / most);
+    return (int)((w->NG + *per - 1) / *per);
+}
+
+template <int TT, bool FUSED>
+int launch_few(llmq_ctx *ctx, const Product &p, const llmq_mat *w, size_t front) {
+    int per;
+    const int waves = few_waves(w, few_most(TT), &per);
+    const size_t sums = (size_t)waves * TT * 1024;
+    const dim3 grid((unsigned)w->ntiles, (unsigned)((p.T + 16 * TT - 1) / (16 * TT)));
+    hipLaunchKernelGGL((mx4_few_kernel<TT, FUSED>), grid, dim3(64 * waves), sums > front ? sums : front, ctx->stream, p,
+                       per);
     LLMQ_HIP(hipGetLastError());
     return LLMQ_OK;
+}
+
+// The product of quantized tokens, or (codes null) of one token's floats x.
+int launch_product(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scales, const float *x, const llmq_mat *w,
+                   int64_t T, float *out, const float *bias, int flags) {
+    Product p;
+    p.xc = codes;
+    p.xs = scales;
+    p.x = x;
+    p.wc = w->codes;
+    p.ws = reinterpret_cast<const uint32_t *>(w->scales);
+    p.T = T;
+    p.n = (int)w->n;
+    p.nb = (int)(w->k / 32);
+    p.steps = (int)w->CK;
+    p.words = (int)w->NG;
+    p.ntiles = (int)w->ntiles;
+    p.out = out;
+    p.bias = bias;
+    p.flags = flags;
+    if (!codes) return launch_few<1, true>(ctx, p, w, (size_t)w->NG * (16 + 256));
+    if (T >= kMany) {
+        const int64_t gx = (w->n + kOuts - 1) / kOuts, gy = (T + kTokens - 1) / kTokens;
+        LLMQ_REQUIRE(gx * gy <= INT32_MAX, "mx4_linear: %lld tokens by %lld outputs", (long long)T, (long long)w->n);
+        hipLaunchKernelGGL(mx4_many_kernel, dim3((unsigned)(gx * gy)), dim3(256), 0, ctx->stream, p, (int)gx, (int)gy);
+        LLMQ_HIP(hipGetLastError());
+        return LLMQ_OK;
+    }
+    if (T <= 16) return launch_few<1, false>(ctx, p, w, 0);
+    if (T <= 32) return launch_few<2, false>(ctx, p, w, 0);
+    return launch_few<4, false>(ctx, p, w, 0);
 }
 
 int check_epilogue(const char *name, const float *out, const float *bias, int64_t T, int flags) {
@@ -244,6 +618,8 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
     LLMQ_REQUIRE(T >= 0 && T <= INT32_MAX && (x || T == 0), "linear: %lld microscaled tokens", (long long)T);
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
+    // one token's row fits LDS beside the sums
+    if (T == 1 && w->NG * (16 + 256) <= 65536) return launch_product(ctx, nullptr, nullptr, x, w, 1, out, bias, flags);
     const int64_t need = mx4_record_bytes(T, w->k);
     if (rec_cap < 0) {
         // the workspace is one for the context: two graphs that held it could not run side by side
@@ -257,14 +633,14 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
     }
     uint8_t *codes = static_cast<uint8_t *>(rec), *scales = codes + ((T * w->k / 2 + 255) & ~(int64_t)255);
     RC(launch_quantize(ctx, x, w->k, T, w->k, codes, scales));
-    return launch_product(ctx, codes, scales, w, T, out, bias, flags);
+    return launch_product(ctx, codes, scales, nullptr, w, T, out, bias, flags);
 }
 
 int mx4_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *dst) {
     DeviceGuard guard(ctx);
     const int64_t nb = m->k / 32, tile = row >> 4, r = row & 15;
-    std::vector<uint8_t> c((size_t)m->CK * 1024), s((size_t)m->NG * 256);
-    LLMQ_HIP(hipMemcpyAsync(c.data(), m->codes + tile * m->CK * 1024, c.size(), hipMemcpyDeviceToHost, ctx->stream));
+    std::vector<uint8_t> c((size_t)m->NG * 4096), s((size_t)m->NG * 256);
+    LLMQ_HIP(hipMemcpyAsync(c.data(), m->codes + tile * m->NG * 4096, c.size(), hipMemcpyDeviceToHost, ctx->stream));
     LLMQ_HIP(hipMemcpyAsync(s.data(), reinterpret_cast<const uint8_t *>(m->scales) + tile * m->NG * 256, s.size(),
                             hipMemcpyDeviceToHost, ctx->stream));
     LLMQ_HIP(hipStreamSynchronize(ctx->stream));
@@ -297,10 +673,10 @@ int llmq_mx4_dequantize(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scal
     LLMQ_REQUIRE(ldo >= K, "mx4_dequantize: rows of %lld floats %lld apart", (long long)K, (long long)ldo);
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
-    const int64_t nb = K / 32, total = T * nb, grid = (total + 255) / 256;
-    LLMQ_REQUIRE(grid <= INT32_MAX, "mx4_dequantize: %lld rows of %lld", (long long)T, (long long)K);
-    hipLaunchKernelGGL(mx4_dequantize_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, codes, scales, nb, total,
-                       out, ldo);
+    Quarters u;
+    RC(quarters("mx4_dequantize", T, K, ldo, &u));
+    hipLaunchKernelGGL(mx4_dequantize_kernel, dim3((unsigned)u.grid), dim3(256), 0, ctx->stream,
+                       reinterpret_cast<const uint32_t *>(codes), scales, u.unit, u.total, out, ldo);
     LLMQ_HIP(hipGetLastError());
     return LLMQ_OK;
 }
@@ -316,7 +692,7 @@ int llmq_mat_from_f32_mx4_device(llmq_ctx *ctx, const float *src, int64_t rows, 
     llmq_mat *m = nullptr;
     RC(mx4_alloc(ctx, n, k, &m));
     hipLaunchKernelGGL(mx4_weights_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, src, cols, reduce_rows, n,
-                       nb, m->CK, m->NG, reinterpret_cast<uint4 *>(m->codes), reinterpret_cast<uint8_t *>(m->scales));
+                       nb, m->NG, reinterpret_cast<uint4 *>(m->codes), reinterpret_cast<uint8_t *>(m->scales));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         llmq_mat_free(m);
@@ -356,7 +732,7 @@ int llmq_mat_restore_mx4(llmq_ctx *ctx, int64_t rows, int64_t cols, const uint8_
     int rc = LLMQ_OK;
     try {
         const int64_t nb = cols / 32;
-        std::vector<uint8_t> c((size_t)(m->ntiles * m->CK) * 1024, 0), s((size_t)(m->ntiles * m->NG) * 256, 127);
+        std::vector<uint8_t> c((size_t)(m->ntiles * m->NG) * 4096, 0), s((size_t)(m->ntiles * m->NG) * 256, 127);
         for (int64_t o = 0; o < rows; o++)
             for (int64_t b = 0; b < nb; b++) {
                 const Place at = place_of(m, o, b);
@@ -382,7 +758,7 @@ int llmq_mat_export_mx4(llmq_ctx *ctx, const llmq_mat *m, uint8_t *codes, uint8_
     LLMQ_REQUIRE(ctx && m && m->kind == MAT_MX4, "export_mx4: not a microscaled matrix");
     DeviceGuard guard(ctx);
     try {
-        std::vector<uint8_t> c((size_t)(m->ntiles * m->CK) * 1024), s((size_t)(m->ntiles * m->NG) * 256);
+        std::vector<uint8_t> c((size_t)(m->ntiles * m->NG) * 4096), s((size_t)(m->ntiles * m->NG) * 256);
         LLMQ_HIP(hipMemcpyAsync(c.data(), m->codes, c.size(), hipMemcpyDeviceToHost, ctx->stream));
         LLMQ_HIP(hipMemcpyAsync(s.data(), m->scales, s.size(), hipMemcpyDeviceToHost, ctx->stream));
         LLMQ_HIP(hipStreamSynchronize(ctx->stream));
@@ -409,7 +785,7 @@ int llmq_mx4_linear(llmq_ctx *ctx, float *out, const uint8_t *codes, const uint8
     RC(check_epilogue("mx4_linear", out, bias, T, flags));
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
-    return launch_product(ctx, codes, scales, w, T, out, bias, flags);
+    return launch_product(ctx, codes, scales, nullptr, w, T, out, bias, flags);
 }
 
 }  // extern "C"

@@ -391,17 +391,15 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     uint32_t kr[NT * NC][4], vr[ND][NV];
     v4f ks[NT], vs[NT];
     int64_t at = 0;  // the block's first row
-    int bytes = kBytes;  // of its keys, and of its values: none of a page that is none, whose loads give zeros
     auto find = [&]() -> int {
         const int page = table_at(table + __builtin_amdgcn_readfirstlane(pi));
         const bool ok = page >= 0 && page < c.pages;
         at = uniform64(((int64_t)(ok ? page : 0) * c.n_kv + kvh) * c.page + off * B);
-        bytes = __builtin_amdgcn_readfirstlane(ok ? kBytes : 0);
         const int64_t left = len - (int64_t)b * B;
         return __builtin_amdgcn_readfirstlane(ok ? (int)(left < B ? left : B) : 0);
     };
     auto load_k = [&]() {
-        const auto rk = llmq_rsrc(c.k + at * HD * ELEM, bytes);
+        const auto rk = llmq_rsrc(c.k + at * HD * ELEM, kBytes);
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -412,14 +410,14 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
                 for (int e = 0; e < 4; e++) kr[t * NC + i][e] = y[e];
             }
         if constexpr (ELEM == 1) {
-            const auto rs = llmq_rsrc(c.ks + at, bytes < 4 * B ? bytes : 4 * B);
+            const auto rs = llmq_rsrc(c.ks + at, 4 * B);
 #pragma unroll
             for (int t = 0; t < NT; t++)
                 ks[t] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * q, 64 * t, 0));
         }
     };
     auto load_v = [&]() {
-        const auto rv = llmq_rsrc(c.v + at * HD * ELEM, bytes);
+        const auto rv = llmq_rsrc(c.v + at * HD * ELEM, kBytes);
 #pragma unroll
         for (int d = 0; d < ND; d++) {
             const int vo = (n * B + q * 8) * ELEM, so = d * 16 * B * ELEM;
@@ -434,7 +432,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
             }
         }
         if constexpr (ELEM == 1) {
-            const auto rs = llmq_rsrc(c.vs + at, bytes < 4 * B ? bytes : 4 * B);
+            const auto rs = llmq_rsrc(c.vs + at, 4 * B);
 #pragma unroll
             for (int t = 0; t < NT; t++)
                 vs[t] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * q, 64 * t, 0));
@@ -588,9 +586,15 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
 #pragma unroll
             for (int i = 0; i < NT * 4; i++) sv[i] = fmaf(slope, base + (float)(16 * (i >> 2) + (i & 3)), sv[i]);
         }
-        if (!LAST && have == 0)
+        if (!LAST && have == 0) {
 #pragma unroll
             for (int i = 0; i < NT * 4; i++) sv[i] = -INFINITY;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int i = 0; i < NV; i++) vr[d][i] = 0;
+            if constexpr (ELEM == 1) vs[0] = vs[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        }
         if (LAST && have < B) {
 #pragma unroll
             for (int i = 0; i < NT * 4; i++) {
