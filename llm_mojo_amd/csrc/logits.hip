@@ -2,18 +2,19 @@
 // llmq_adjust_logits): penalties for tokens a sequence holds already, biases,
 // a grammar's mask.
 //
-// One pass over the logits.  A workgroup takes a row's next kChunk entries
-// and counts the history's tokens that fall there in LDS (integer adds: the
-// order does not matter), so no table of counts goes through memory; a
-// history is read once a chunk, from the caches after the first.
+// One pass over the logits, bound by reading and writing them.  A workgroup
+// takes a row's next CHUNK entries into registers and, while they are on
+// their way, counts the history's tokens that fall there in LDS (integer
+// adds: the order does not matter), so no table of counts goes through
+// memory; a history is read once a chunk, from the caches after the first.
 #include <math.h>
 
 #include "common.h"
 
 namespace {
 
-constexpr int kChunk = 4096, kThreads = 256;
-constexpr int kPer = kChunk / kThreads;
+constexpr int kThreads = 256;
+constexpr int kSmall = 1024, kLarge = 4096;  // entries of a workgroup
 
 struct Rules {
     const int32_t *hist;
@@ -63,51 +64,128 @@ __device__ __forceinline__ Best block_best(Best b, Best *red) {
     return b;
 }
 
-__global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *__restrict__ in, int64_t ldi,
-                                                                 float *__restrict__ out, int64_t ldo, int V, Rules u,
-                                                                 Best *__restrict__ parts) {
-    __shared__ int count[kChunk];
-    __shared__ float add[kChunk];
+struct Float4 {
+    float x[4];
+} __attribute__((packed, aligned(4)));
+
+template <int CHUNK>
+__global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in, int64_t ldi, float *out, int64_t ldo,
+                                                                 int V, Rules u, Best *__restrict__ parts) {
+    constexpr int N = CHUNK / (4 * kThreads);  // fours of entries a thread
+    __shared__ __align__(16) int count[CHUNK];
+    __shared__ __align__(16) float add[CHUNK];
+    __shared__ int ids[kThreads], from[kThreads / 64];
+    __shared__ float val[kThreads];
     __shared__ Best red[kThreads / 64];
     const int64_t r = blockIdx.y;
-    const int v0 = blockIdx.x * kChunk, tid = threadIdx.x;
-    for (int i = tid; i < kChunk; i += kThreads) {
-        count[i] = 0;
-        add[i] = 0.0f;
-    }
-    __syncthreads();
-    if (u.hist) {
-        const Span s = span_of(u.hist_off, u.hist_len, r);
-        for (int64_t i = s.lo + tid; i < s.hi; i += kThreads) {
-            const uint32_t at = (uint32_t)u.hist[i] - (uint32_t)v0;
-            if (at < (uint32_t)kChunk) atomicAdd(&count[at], 1);
+    const int v0 = blockIdx.x * CHUNK, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const float *src = in + r * ldi;
+    Float4 x[N];
+    uint32_t bits[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int v = v0 + 4 * (tid + kThreads * k);
+        bits[k] = 15;
+        if (v + 4 <= V) {
+            x[k] = *reinterpret_cast<const Float4 *>(src + v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[k].x[i] = v + i < V ? src[v + i] : 0.0f;
         }
+        if (u.mask && v < V) bits[k] = u.mask[r * u.mask_ld + (v >> 5)] >> (v & 31);
     }
-    // biases of one token in the list's order: one thread adds them all
-    if (u.bias_ids && tid == 0) {
-        const Span s = span_of(u.bias_off, u.bias_len, r);
-        for (int64_t i = s.lo; i < s.hi; i++) {
-            const uint32_t at = (uint32_t)u.bias_ids[i] - (uint32_t)v0;
-            if (at < (uint32_t)kChunk) add[at] += u.bias[i];
-        }
-    }
-    __syncthreads();
     const float rep = u.rep ? u.rep[r] : 1.0f, pres = u.pres ? u.pres[r] : 0.0f, freq = u.freq ? u.freq[r] : 0.0f;
-    Best b{-INFINITY, INT32_MAX};
-    for (int i = tid; i < kChunk && v0 + i < V; i += kThreads) {
-        const int v = v0 + i;
-        float l = in[r * ldi + v];
-        const int c = count[i];
-        if (c > 0) {
-            if (u.rep) l = l > 0.0f ? l / rep : l * rep;
-            l = l - (freq * (float)c + pres);
+    const Span hist = u.hist ? span_of(u.hist_off, u.hist_len, r) : Span{0, 0};
+    const Span bias = u.bias_ids ? span_of(u.bias_off, u.bias_len, r) : Span{0, 0};
+    if (hist.lo < hist.hi || bias.lo < bias.hi) {  // the same for the whole workgroup
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            reinterpret_cast<int4 *>(count)[tid + kThreads * k] = make_int4(0, 0, 0, 0);
+            reinterpret_cast<float4 *>(add)[tid + kThreads * k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        if (u.bias_ids) l = l + add[i];
-        if (u.mask && !((u.mask[r * u.mask_ld + (v >> 5)] >> (v & 31)) & 1)) l = -INFINITY;
-        out[r * ldo + v] = l;
-        if (l > b.v) {  // never for NaN and -inf
-            b.v = l;
-            b.i = v;
+        __syncthreads();
+        for (int64_t i = hist.lo + tid; i < hist.hi; i += kThreads) {
+            const uint32_t at = (uint32_t)u.hist[i] - (uint32_t)v0;
+            if (at < (uint32_t)CHUNK) atomicAdd(&count[at], 1);
+        }
+        // biases, a batch of kThreads at a time: those of this chunk go to
+        // LDS in the list's order, and the first of each token adds up all
+        // of its token's in that order
+        for (int64_t i0 = bias.lo; i0 < bias.hi; i0 += kThreads) {
+            const bool have = i0 + tid < bias.hi;
+            const uint32_t at = have ? (uint32_t)u.bias_ids[i0 + tid] - (uint32_t)v0 : 0xffffffffu;
+            const float b = have ? u.bias[i0 + tid] : 0.0f;
+            const bool in_chunk = at < (uint32_t)CHUNK;
+            const uint64_t who = __ballot(in_chunk);
+            if (lane == 0) from[w] = __popcll(who);
+            __syncthreads();
+            int n = 0, first = 0;
+#pragma unroll
+            for (int k = 0; k < kThreads / 64; k++) {
+                if (k == w) first = n;
+                n += from[k];
+            }
+            if (in_chunk) {
+                const int k = first + __popcll(who & ((1ull << lane) - 1));
+                ids[k] = (int)at;
+                val[k] = b;
+            }
+            __syncthreads();
+            if (tid < n) {
+                const int mine = ids[tid];
+                bool lead = true;
+                for (int k = 0; k < tid; k++) lead &= ids[k] != mine;
+                if (lead) {
+                    float s = add[mine];
+                    for (int k = tid; k < n; k++)
+                        if (ids[k] == mine) s += val[k];
+                    add[mine] = s;
+                }
+            }
+            __syncthreads();
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int4 c4 = reinterpret_cast<const int4 *>(count)[tid + kThreads * k];
+            const float4 a4 = reinterpret_cast<const float4 *>(add)[tid + kThreads * k];
+            const int c[4] = {c4.x, c4.y, c4.z, c4.w};
+            const float a[4] = {a4.x, a4.y, a4.z, a4.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float l = x[k].x[i];
+                if (c[i] > 0) {
+                    if (u.rep) l = l > 0.0f ? l / rep : l * rep;
+                    l = l - (freq * (float)c[i] + pres);
+                }
+                x[k].x[i] = u.bias_ids ? l + a[i] : l;
+            }
+        }
+    } else if (u.bias_ids) {  // what adding no bias does: -0 becomes 0
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[k].x[i] += 0.0f;
+    }
+    Best b{-INFINITY, INT32_MAX};
+    float *dst = out + r * ldo;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int v = v0 + 4 * (tid + kThreads * k);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (!((bits[k] >> i) & 1)) x[k].x[i] = -INFINITY;
+            if (x[k].x[i] > b.v && v + i < V) {  // never for NaN and -inf
+                b.v = x[k].x[i];
+                b.i = v + i;
+            }
+        }
+        if (v + 4 <= V) {
+            *reinterpret_cast<Float4 *>(dst + v) = x[k];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (v + i < V) dst[v + i] = x[k].x[i];
         }
     }
     if (!parts) return;
@@ -127,11 +205,19 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Best *__restrict__
 
 }  // namespace
 
+namespace {
+
+// Small chunks where large ones would leave CUs without a workgroup.
+int chunk_of(int64_t rows, int64_t V) { return rows * ((V + kLarge - 1) / kLarge) < 512 ? kSmall : kLarge; }
+
+}  // namespace
+
 extern "C" {
 
 int64_t llmq_adjust_logits_work_bytes(int64_t rows, int64_t V) {
     if (rows < 0 || rows > 65535 || V <= 0 || V > INT32_MAX / 2) return -1;
-    return rows * ((V + kChunk - 1) / kChunk) * (int64_t)sizeof(Best) + 16;
+    const int chunk = chunk_of(rows, V);
+    return rows * ((V + chunk - 1) / chunk) * (int64_t)sizeof(Best) + 16;
 }
 
 int llmq_adjust_logits(llmq_ctx *ctx, float *out, int64_t ldo, const float *logits, int64_t ldl, int64_t rows,
@@ -161,10 +247,11 @@ int llmq_adjust_logits(llmq_ctx *ctx, float *out, int64_t ldo, const float *logi
                  (long long)work_bytes, (long long)want);
     if (rows == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
-    const int n = (int)((V + kChunk - 1) / kChunk);
+    const int chunk = chunk_of(rows, V), n = (int)((V + chunk - 1) / chunk);
     Best *parts = pick ? static_cast<Best *>(work) : nullptr;
-    hipLaunchKernelGGL(adjust_logits_kernel, dim3((unsigned)n, (unsigned)rows), dim3(kThreads), 0, ctx->stream, logits,
-                       ldl, out, ldo, (int)V, u, parts);
+    auto kernel = chunk == kSmall ? adjust_logits_kernel<kSmall> : adjust_logits_kernel<kLarge>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n, (unsigned)rows), dim3(kThreads), 0, ctx->stream, logits, ldl, out, ldo,
+                       (int)V, u, parts);
     if (pick)
         hipLaunchKernelGGL(pick_kernel, dim3((unsigned)rows), dim3(kThreads), 0, ctx->stream, parts, n, pick);
     LLMQ_HIP(hipGetLastError());

@@ -44,26 +44,16 @@ __device__ __forceinline__ int64_t head_row(const Layer &c, int page, int head) 
     return ((int64_t)page * c.n_kv + head) * c.page;
 }
 
-// QuantKV.store's quantisation of one row (kvcache.mojo:333-342) over a wave,
-// HD / 64 dimensions a lane: s = max|x| / 127 (1 for a row of zeros), codes
-// round(x / s) away from zero at ties.  A row with a NaN or an infinity gets
-// the scale NaN; one below 2^-120, whose reciprocal scale is infinite, is a row of zeros.
-template <int HD>
-__device__ __forceinline__ float quant_row(const float (&x)[HD / 64], int (&code)[HD / 64]) {
-    float m = 0.0f, bad = 0.0f;
-#pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        m = fmaxf(m, fabsf(x[i]));
-        bad += x[i] - x[i];  // NaN for NaN and infinities
-    }
-    m = llmq_wave_max_all(m);
-    const bool none = __any(bad != 0.0f || bad != bad);
-    const float s = m < 0x1p-120f ? 1.0f : m / 127.0f;
-    const float inv = 1.0f / s;
-#pragma unroll
-    for (int i = 0; i < HD / 64; i++) code[i] = none ? 0 : llmq_to_int(roundf(x[i] * inv));
-    return none ? __uint_as_float(0x7fc00000u) : s;
+// QuantKV.store's quantisation of a row (kvcache.mojo:333-342): s = max|x| /
+// 127 (1 for a row of zeros), codes round(x / s) away from zero at ties, kept
+// plus kBias.  A row with a NaN or an infinity (largest: infinity) gets the
+// scale NaN; one below 2^-120, whose reciprocal scale is infinite, is a row of
+// zeros.
+__device__ __forceinline__ float row_scale(float largest) {
+    if (largest == INFINITY) return __uint_as_float(0x7fc00000u);
+    return largest < 0x1p-120f ? 1.0f : largest / 127.0f;
 }
+__device__ __forceinline__ int row_code(float x, float inv) { return llmq_to_int(roundf(x * inv)) + kBias; }
 
 __device__ __forceinline__ uint16_t half_bits(float x) {
     // nearest even; finite values past the range become its ends
@@ -71,13 +61,20 @@ __device__ __forceinline__ uint16_t half_bits(float x) {
     return __half_as_ushort(__float2half_rn(lim));
 }
 
-// A row's codes (int8 with kBias, or float16 bits) and scale, dimensions lane + 64 i.
+// A row's codes (int8, or float16 bits) and scale, dimensions lane + 64 i.
 template <int HD, int ELEM>
 __device__ __forceinline__ float encode_row(const float (&x)[HD / 64], int (&code)[HD / 64]) {
     if constexpr (ELEM == 1) {
-        const float s = quant_row<HD>(x, code);
+        float m = 0.0f, bad = 0.0f;
 #pragma unroll
-        for (int i = 0; i < HD / 64; i++) code[i] += kBias;
+        for (int i = 0; i < HD / 64; i++) {
+            m = fmaxf(m, fabsf(x[i]));
+            bad += x[i] - x[i];  // NaN for NaN and infinities
+        }
+        m = llmq_wave_max_all(bad != 0.0f || bad != bad ? INFINITY : m);
+        const float s = row_scale(m), inv = 1.0f / s;
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) code[i] = row_code(x[i], inv);
         return s;
     } else {
 #pragma unroll
@@ -125,58 +122,166 @@ __device__ __forceinline__ NewRow<HD, ELEM> store_row(const Layer &c, int page, 
     return x;
 }
 
-// Element (lane + 64 i) of a cached key / value row.
+// Rows of a call to or from the cache: a workgroup kRows rows of one head,
+// eight lanes a row, the values through LDS so that both sides see whole
+// lines: the floats a row at a time, the cache a dimension's slots at a time
+// (neighbouring rows are mostly neighbouring positions).
+constexpr int kRows = 32, kLanes = 8;
+
+// Where row t's position is: its first element in the keys (units of rows),
+// and in the values the element of dimension 0; -1: nowhere.
+struct Dest {
+    int64_t row, value;
+};
+template <int HD>
+__device__ __forceinline__ Dest dest_of(const Layer &c, const int32_t *seq, const int32_t *pos, int64_t n_seq,
+                                        int64_t t, int64_t T, int head) {
+    Dest d{-1, -1};
+    if (t >= T) return d;
+    const int s = seq[t], p = pos[t];
+    if (s < 0 || s >= n_seq) return d;
+    const int page = pkv::page_of(c.table + s * c.width, c.width, c.page, c.pages, p);
+    if (page < 0) return d;
+    const int off = p % c.page;
+    d.row = head_row(c, page, head) + off;
+    d.value = (d.row - off % B) * HD + pkv::value_slot(off % B);
+    return d;
+}
+
+// Maximum over the eight lanes of a row.
+__device__ __forceinline__ float eighth_max(float v) {
+    v = fmaxf(v, llmq_dppf<0xB1>(v));
+    v = fmaxf(v, llmq_dppf<0x4E>(v));
+    return fmaxf(v, llmq_dppf<0x141>(v));  // row_half_mirror
+}
+
+struct Floats4 {
+    float x[4];
+} __attribute__((packed, aligned(4)));
+
+// llmq_pkv_store.
 template <int HD, int ELEM>
-__device__ __forceinline__ void load_row(const Layer &c, int page, int off, int head, float (&k)[HD / 64],
-                                         float (&v)[HD / 64], int lane) {
-    const int64_t row = head_row(c, page, head) + off;
-    const int64_t vrow = (head_row(c, page, head) + off / B * B) * HD;
-    const int slot = pkv::value_slot(off % B);
+__global__ __launch_bounds__(kRows *kLanes) void pkv_store_kernel(Layer c, const float *__restrict__ k,
+                                                                  const float *__restrict__ v, int64_t ld, int64_t T,
+                                                                  const int32_t *__restrict__ seq,
+                                                                  const int32_t *__restrict__ pos, int64_t n_seq) {
+    constexpr int NP = HD / 32, STRIDE = HD * ELEM + 4;  // fours of a lane; bytes of a row in LDS
+    __shared__ __align__(4) uint8_t vt[kRows * STRIDE];
+    __shared__ int64_t at[kRows];
+    const int tid = threadIdx.x, row = tid / kLanes, j = tid % kLanes, head = blockIdx.y;
+    const int64_t t = (int64_t)blockIdx.x * kRows + row;
+    const Dest d = dest_of<HD>(c, seq, pos, n_seq, t, T, head);
+    if (j == 0) at[row] = d.value;
+    if (d.row >= 0) {
+        const float *src[2] = {k + t * ld + head * HD, v + t * ld + head * HD};
+        float x[2][NP][4];
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        const int d = lane + 64 * i;
-        if constexpr (ELEM == 1) {
-            k[i] = (float)((int)c.k[row * HD + d] - kBias) * c.ks[row];
-            v[i] = (float)((int)c.v[vrow + (int64_t)d * B + slot] - kBias) * c.vs[row];
-        } else {
-            k[i] = __half2float(__ushort_as_half(reinterpret_cast<const uint16_t *>(c.k)[row * HD + d]));
-            v[i] = __half2float(
-                __ushort_as_half(reinterpret_cast<const uint16_t *>(c.v)[vrow + (int64_t)d * B + slot]));
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < NP; i++)
+                *reinterpret_cast<Floats4 *>(x[s][i]) = *reinterpret_cast<const Floats4 *>(src[s] + 32 * i + 4 * j);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            uint8_t *keys = s == 0 ? c.k + d.row * HD * ELEM : vt + row * STRIDE;
+            if constexpr (ELEM == 1) {
+                float m = 0.0f, bad = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NP; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        m = fmaxf(m, fabsf(x[s][i][e]));
+                        bad += x[s][i][e] - x[s][i][e];  // NaN for NaN and infinities
+                    }
+                m = eighth_max(bad != 0.0f || bad != bad ? INFINITY : m);
+                const float scale = row_scale(m), inv = 1.0f / scale;
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    uint32_t u = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) u |= (uint32_t)row_code(x[s][i][e], inv) << (8 * e);
+                    *reinterpret_cast<uint32_t *>(keys + 32 * i + 4 * j) = u;
+                }
+                if (j == 0) (s == 0 ? c.ks : c.vs)[d.row] = scale;
+            } else {
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    uint32_t *u = reinterpret_cast<uint32_t *>(keys + 64 * i + 8 * j);
+                    u[0] = half_bits(x[s][i][0]) | (uint32_t)half_bits(x[s][i][1]) << 16;
+                    u[1] = half_bits(x[s][i][2]) | (uint32_t)half_bits(x[s][i][3]) << 16;
+                }
+            }
         }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < kRows * HD; i += kRows * kLanes) {
+        const int e = i % kRows, dim = i / kRows;
+        if (at[e] < 0) continue;
+        if constexpr (ELEM == 1)
+            c.v[at[e] + dim * B] = vt[e * STRIDE + dim];
+        else
+            reinterpret_cast<uint16_t *>(c.v)[at[e] + dim * B] =
+                *reinterpret_cast<const uint16_t *>(vt + e * STRIDE + 2 * dim);
     }
 }
 
-// llmq_pkv_store: one wave a (token, head).
+// llmq_pkv_fetch; zeros where the cache has no row.
 template <int HD, int ELEM>
-__global__ __launch_bounds__(64) void pkv_store_kernel(Layer c, const float *__restrict__ k,
-                                                       const float *__restrict__ v, int64_t ld,
-                                                       const int32_t *__restrict__ seq,
-                                                       const int32_t *__restrict__ pos, int64_t n_seq) {
-    const int64_t t = blockIdx.x;
-    const int head = blockIdx.y, s = seq[t];
-    if (s < 0 || s >= n_seq) return;
-    const int page = pkv::page_of(c.table + s * c.width, c.width, c.page, c.pages, pos[t]);
-    if (page < 0) return;
-    store_row<HD, ELEM>(c, page, pos[t] % c.page, head, k + t * ld + head * HD, v + t * ld + head * HD, threadIdx.x);
-}
-
-// llmq_pkv_fetch: one wave a (token, head); zeros where the cache has no row.
-template <int HD, int ELEM>
-__global__ __launch_bounds__(64) void pkv_fetch_kernel(Layer c, float *__restrict__ k, float *__restrict__ v,
-                                                       int64_t ld, const int32_t *__restrict__ seq,
-                                                       const int32_t *__restrict__ pos, int64_t n_seq) {
-    const int64_t t = blockIdx.x;
-    const int head = blockIdx.y, s = seq[t], lane = threadIdx.x;
-    int page = -1;
-    if (s >= 0 && s < n_seq) page = pkv::page_of(c.table + s * c.width, c.width, c.page, c.pages, pos[t]);
-    float kx[HD / 64], vx[HD / 64];
+__global__ __launch_bounds__(kRows *kLanes) void pkv_fetch_kernel(Layer c, float *__restrict__ k,
+                                                                  float *__restrict__ v, int64_t ld, int64_t T,
+                                                                  const int32_t *__restrict__ seq,
+                                                                  const int32_t *__restrict__ pos, int64_t n_seq) {
+    constexpr int NP = HD / 32, STRIDE = HD * ELEM + 4;
+    __shared__ __align__(4) uint8_t vt[kRows * STRIDE];
+    __shared__ int64_t at[kRows];
+    const int tid = threadIdx.x, row = tid / kLanes, j = tid % kLanes, head = blockIdx.y;
+    const int64_t t = (int64_t)blockIdx.x * kRows + row;
+    const Dest d = dest_of<HD>(c, seq, pos, n_seq, t, T, head);
+    if (j == 0) at[row] = d.value;
+    uint32_t key[NP][ELEM];
+    float ks = 1.0f, vs = 1.0f;
+    if (d.row >= 0) {
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) kx[i] = vx[i] = 0.0f;
-    if (page >= 0) load_row<HD, ELEM>(c, page, pos[t] % c.page, head, kx, vx, lane);
+        for (int i = 0; i < NP; i++)
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        k[t * ld + head * HD + lane + 64 * i] = kx[i];
-        v[t * ld + head * HD + lane + 64 * i] = vx[i];
+            for (int e = 0; e < ELEM; e++)
+                key[i][e] = *reinterpret_cast<const uint32_t *>(c.k + (d.row * HD + 32 * i + 4 * j) * ELEM + 4 * e);
+        if constexpr (ELEM == 1) {
+            ks = c.ks[d.row];
+            vs = c.vs[d.row];
+        }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < kRows * HD; i += kRows * kLanes) {
+        const int e = i % kRows, dim = i / kRows;
+        if (at[e] < 0) continue;
+        if constexpr (ELEM == 1)
+            vt[e * STRIDE + dim] = c.v[at[e] + dim * B];
+        else
+            *reinterpret_cast<uint16_t *>(vt + e * STRIDE + 2 * dim) =
+                reinterpret_cast<const uint16_t *>(c.v)[at[e] + dim * B];
+    }
+    __syncthreads();
+    if (t >= T) return;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        Floats4 x{}, y{};
+        if (d.row >= 0)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int dim = 32 * i + 4 * j + e;
+                if constexpr (ELEM == 1) {
+                    x.x[e] = (float)((int)((key[i][0] >> (8 * e)) & 255) - kBias) * ks;
+                    y.x[e] = (float)((int)vt[row * STRIDE + dim] - kBias) * vs;
+                } else {
+                    x.x[e] = __half2float(__ushort_as_half((uint16_t)(key[i][e >> 1] >> (16 * (e & 1)))));
+                    y.x[e] = __half2float(
+                        __ushort_as_half(*reinterpret_cast<const uint16_t *>(vt + row * STRIDE + 2 * dim)));
+                }
+            }
+        *reinterpret_cast<Floats4 *>(k + t * ld + head * HD + 32 * i + 4 * j) = x;
+        *reinterpret_cast<Floats4 *>(v + t * ld + head * HD + 32 * i + 4 * j) = y;
     }
 }
 
@@ -897,8 +1002,8 @@ int llmq_pkv_store(llmq_ctx *ctx, llmq_pkv *kv, int layer, const float *k, const
     const Layer c = layer_of(kv, layer, table, width);
     return dispatch(kv, [&](auto hd, auto elem) -> int {
         hipLaunchKernelGGL((pkv_store_kernel<decltype(hd)::value, decltype(elem)::value>),
-                           dim3((unsigned)T, (unsigned)kv->n_kv), dim3(64), 0, ctx->stream, c, k, v, ld, seq, pos,
-                           n_seq);
+                           dim3((unsigned)((T + kRows - 1) / kRows), (unsigned)kv->n_kv), dim3(kRows * kLanes), 0,
+                           ctx->stream, c, k, v, ld, T, seq, pos, n_seq);
         LLMQ_HIP(hipGetLastError());
         return LLMQ_OK;
     });
@@ -913,8 +1018,8 @@ int llmq_pkv_fetch(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *k, float
     const Layer c = layer_of(kv, layer, table, width);
     return dispatch(kv, [&](auto hd, auto elem) -> int {
         hipLaunchKernelGGL((pkv_fetch_kernel<decltype(hd)::value, decltype(elem)::value>),
-                           dim3((unsigned)T, (unsigned)kv->n_kv), dim3(64), 0, ctx->stream, c, k, v, ld, seq, pos,
-                           n_seq);
+                           dim3((unsigned)((T + kRows - 1) / kRows), (unsigned)kv->n_kv), dim3(kRows * kLanes), 0,
+                           ctx->stream, c, k, v, ld, T, seq, pos, n_seq);
         LLMQ_HIP(hipGetLastError());
         return LLMQ_OK;
     });
