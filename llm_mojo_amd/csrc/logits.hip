@@ -14,7 +14,8 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSmall = 1024, kLarge = 4096;  // entries of a workgroup
+constexpr int kAhead = 8;  // entries of the history a thread asks for at once
+constexpr int kSmall = 1024, kLarge = 2048;  // entries of a workgroup
 
 struct Rules {
     const int32_t *hist;
@@ -97,6 +98,18 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
     const float rep = u.rep ? u.rep[r] : 1.0f, pres = u.pres ? u.pres[r] : 0.0f, freq = u.freq ? u.freq[r] : 0.0f;
     const Span hist = u.hist ? span_of(u.hist_off, u.hist_len, r) : Span{0, 0};
     const Span bias = u.bias_ids ? span_of(u.bias_off, u.bias_len, r) : Span{0, 0};
+    // the lists' first entries too, before anything waits
+    int32_t h[kAhead], bid = -1;
+    float bval = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+        const int64_t i = hist.lo + tid + kThreads * k;
+        h[k] = i < hist.hi ? u.hist[i] : -1;
+    }
+    if (bias.lo + tid < bias.hi) {
+        bid = u.bias_ids[bias.lo + tid];
+        bval = u.bias[bias.lo + tid];
+    }
     if (hist.lo < hist.hi || bias.lo < bias.hi) {  // the same for the whole workgroup
 #pragma unroll
         for (int k = 0; k < N; k++) {
@@ -104,18 +117,25 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
             reinterpret_cast<float4 *>(add)[tid + kThreads * k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         __syncthreads();
-        for (int64_t i = hist.lo + tid; i < hist.hi; i += kThreads) {
-            const uint32_t at = (uint32_t)u.hist[i] - (uint32_t)v0;
+        auto seen = [&](int32_t id) {  // (a negative id is past every chunk)
+            const uint32_t at = (uint32_t)id - (uint32_t)v0;
             if (at < (uint32_t)CHUNK) atomicAdd(&count[at], 1);
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) seen(h[k]);
+        for (int64_t i = hist.lo + tid + kThreads * kAhead; i < hist.hi; i += kThreads) seen(u.hist[i]);
         // biases, a batch of kThreads at a time: those of this chunk go to
         // LDS in the list's order, and the first of each token adds up all
         // of its token's in that order
         for (int64_t i0 = bias.lo; i0 < bias.hi; i0 += kThreads) {
-            const bool have = i0 + tid < bias.hi;
-            const uint32_t at = have ? (uint32_t)u.bias_ids[i0 + tid] - (uint32_t)v0 : 0xffffffffu;
-            const float b = have ? u.bias[i0 + tid] : 0.0f;
+            const uint32_t at = (uint32_t)bid - (uint32_t)v0;
+            const float b = bval;
             const bool in_chunk = at < (uint32_t)CHUNK;
+            bid = -1;
+            if (i0 + kThreads + tid < bias.hi) {
+                bid = u.bias_ids[i0 + kThreads + tid];
+                bval = u.bias[i0 + kThreads + tid];
+            }
             const uint64_t who = __ballot(in_chunk);
             if (lane == 0) from[w] = __popcll(who);
             __syncthreads();
