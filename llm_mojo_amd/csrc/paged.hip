@@ -90,17 +90,12 @@ struct NewRow {
     float ks, vs;
 };
 template <int HD, int ELEM>
-__device__ __forceinline__ NewRow<HD, ELEM> store_row(const Layer &c, int page, int off, int head, const float *k,
-                                                      const float *v, int lane) {
+__device__ __forceinline__ NewRow<HD, ELEM> store_row(const Layer &c, int page, int off, int head,
+                                                      const float (&kx)[HD / 64], const float (&vx)[HD / 64],
+                                                      int lane) {
     const int64_t row = head_row(c, page, head) + off;
     const int64_t vrow = (head_row(c, page, head) + off / B * B) * HD;  // the block's first element
     const int slot = pkv::value_slot(off % B);
-    float kx[HD / 64], vx[HD / 64];
-#pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        kx[i] = k[lane + 64 * i];
-        vx[i] = v[lane + 64 * i];
-    }
     NewRow<HD, ELEM> x;
     x.ks = encode_row<HD, ELEM>(kx, x.k);
     x.vs = encode_row<HD, ELEM>(vx, x.v);
@@ -477,10 +472,14 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         if (b0 == b1) return;  // the same for the whole workgroup
     }
     const int32_t *table = c.table + r * c.width;
-    const int64_t len = uniform64(row_len(c, a, r));
+    const int64_t told = (int64_t)a.len[r] + (a.k ? 1 : 0), len = uniform64(pkv::clamp_len(told, c.width, c.page));
     const int nb = (int)((len + B - 1) / B);
     if (!a.columns) b1 = nb;
     const bool whole = b0 == 0 && b1 == nb;
+    if (b0 == b1) {  // a row of none
+        for (int i = tid; i < hn * HD; i += 64 * pkv::kWaves) a.out[r * a.ldo + (int64_t)h0 * HD + i] = 0.0f;
+        return;
+    }
 
     // the lane's part of its column's query: the column's plane of its dimensions
     float x[NF][8];
@@ -491,8 +490,22 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
             *reinterpret_cast<Float8 *>(x[f]) = *reinterpret_cast<const Float8 *>(
                 src + (ELEM == 1 ? (f >> 1) * 64 + q * 16 + (f & 1) * 8 : f * 32 + q * 8));
     }
+    const bool bias = a.slopes != nullptr;
+    float slope = bias ? a.slopes[h0 + min(n & 7, hn - 1)] : 0.0f;
+    // the new token's row, by the wave whose last block holds it
+    const bool mine = a.k && told == len && b1 == nb && (nb - 1 - b0) % pkv::kWaves == w;
+    float kx[HD / 64], vx[HD / 64];
+    if (mine) {
+        const int64_t from = r * a.ldq + kvh * HD + lane;
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) {
+            kx[i] = a.k[from + 64 * i];
+            vx[i] = a.v[from + 64 * i];
+        }
+    }
     // a block: its page (page 0 in the place of one that is none, with no live positions) and its rows there
-    int b = b0 + w, pi = b / bpp, off = b - pi * bpp;
+    int b = b0 + w;
+    int pi = min(b, b1 - 1) / bpp, off = min(b, b1 - 1) - pi * bpp;
     uint32_t kr[NT * NC][4], vr[ND][NV];
     v4f ks[NT], vs[NT];
     int64_t at = 0;  // the block's first row
@@ -544,12 +557,10 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         }
     };
     // the first block's rows are asked for before the query is taken apart
-    int live = 0;
-    if (b < b1) {
-        live = find();
-        load_k();
-        load_v();
-    }
+    // (a wave without a block asks for another's and leaves them)
+    int live = find();
+    load_k();
+    load_v();
     h8 qf[NF];
     float mul;
     {
@@ -576,22 +587,16 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     const float own = low ? 0x1p-11f : 1.0f, oth = low ? 1.0f : 0x1p-11f;  // a score from the two columns
     const float wg = low ? 2048.0f : 1.0f, wr = low ? -2048.0f : 0.0f;     // a weight to its row's share
     const float icap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-    const bool bias = a.slopes != nullptr;
-    float slope = bias && (n & 7) < hn ? a.slopes[h0 + (n & 7)] : 0.0f;
     asm volatile("" : "+v"(slope));  // waited for here, not behind the loop's loads
 
-    // the new token's row: stored by the wave whose last block holds it
-    // (the tiles of a group store the same bytes), which puts it into
-    // that block as it came from memory
+    // the new token's row goes to the cache (the tiles of a group store the
+    // same bytes), and into the wave's last block as it came from memory
     int fb = -1;
     float fks = 0.0f, fvs = 0.0f;
-    if (a.k && len > 0 && b1 == nb && (nb - 1 - b0) % pkv::kWaves == w) {
-        const int64_t p = len - 1;
-        const int page = a.len[r] == p ? pkv::page_of(table, c.width, c.page, c.pages, p) : -1;
-        if (page >= 0) {
-            const int64_t src = r * a.ldq + kvh * HD;
-            const NewRow<HD, ELEM> y =
-                store_row<HD, ELEM>(c, page, (int)(p % c.page), kvh, a.k + src, a.v + src, lane);
+    if (mine) {
+        const int p = (int)(len - 1), page = table_at(table + __builtin_amdgcn_readfirstlane(p / c.page));
+        if (page >= 0 && page < c.pages) {
+            const NewRow<HD, ELEM> y = store_row<HD, ELEM>(c, page, p % c.page, kvh, kx, vx, lane);
 #pragma unroll
             for (int i = 0; i < HD / 64; i++) {
                 if constexpr (ELEM == 1) {
