@@ -53,9 +53,14 @@ __device__ __forceinline__ void better(Best &a, float v, int i) {
     }
 }
 
-__device__ __forceinline__ Best block_best(Best b, Best *red) {
+__device__ __forceinline__ Best wave_best(Best b) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) better(b, __shfl_xor(b.v, o), __shfl_xor(b.i, o));
+    return b;
+}
+
+__device__ __forceinline__ Best block_best(Best b, Best *red) {
+    b = wave_best(b);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = b;
     __syncthreads();
@@ -213,13 +218,12 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
     if (tid == 0) parts[r * gridDim.x + blockIdx.x] = b;
 }
 
-__global__ __launch_bounds__(kThreads) void pick_kernel(const Best *__restrict__ parts, int n,
-                                                        int64_t *__restrict__ pick) {
-    __shared__ Best red[kThreads / 64];
+// A row's chunks' picks put together: a wave a row.
+__global__ __launch_bounds__(64) void pick_kernel(const Best *__restrict__ parts, int n, int64_t *__restrict__ pick) {
     const Best *p = parts + (int64_t)blockIdx.x * n;
     Best b{-INFINITY, INT32_MAX};
-    for (int i = threadIdx.x; i < n; i += kThreads) better(b, p[i].v, p[i].i);
-    b = block_best(b, red);
+    for (int i = threadIdx.x; i < n; i += 64) better(b, p[i].v, p[i].i);
+    b = wave_best(b);
     if (threadIdx.x == 0) pick[blockIdx.x] = b.i == INT32_MAX ? -1 : b.i;
 }
 
@@ -273,7 +277,7 @@ int llmq_adjust_logits(llmq_ctx *ctx, float *out, int64_t ldo, const float *logi
     hipLaunchKernelGGL(kernel, dim3((unsigned)n, (unsigned)rows), dim3(kThreads), 0, ctx->stream, logits, ldl, out, ldo,
                        (int)V, u, parts);
     if (pick)
-        hipLaunchKernelGGL(pick_kernel, dim3((unsigned)rows), dim3(kThreads), 0, ctx->stream, parts, n, pick);
+        hipLaunchKernelGGL(pick_kernel, dim3((unsigned)rows), dim3(64), 0, ctx->stream, parts, n, pick);
     LLMQ_HIP(hipGetLastError());
     return LLMQ_OK;
 }

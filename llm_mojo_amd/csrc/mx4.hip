@@ -100,36 +100,48 @@ __device__ __forceinline__ uint32_t quant_quarter(const float (&x)[8], int *scal
     return e == 255 ? 0u : codes8(x, inverse_scale(e));
 }
 
-// llmq_mx4_quantize: a lane 8 values, four lanes a block, kQuant blocks'
-// quarters a lane.  Bound by reading the floats; unit = K / 8 lanes a row
-// (one row of them all where the rows lie together).
+// llmq_mx4_quantize: eight lanes a block, 4 values each, so that a wave's load
+// is 1 KB in one piece; kQuant pairs of them a lane.  Two lanes' codes make a
+// word, which the even lane stores for the first of a pair and the odd one
+// for the second.  Bound by reading the floats; unit = K / 4 lanes a row (0:
+// the rows lie together).
 constexpr int kQuant = 4;
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const float *__restrict__ x, int64_t ldx, uint32_t unit,
                                                            int64_t total, uint32_t *__restrict__ codes,
                                                            uint8_t *__restrict__ scales) {
-    const int64_t i0 = (int64_t)blockIdx.x * (256 * kQuant) + threadIdx.x;
-    float v[kQuant][8];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t i0 = ((int64_t)blockIdx.x * 4 + wave) * (128 * kQuant) + lane;
+    Float4 v[2 * kQuant];
 #pragma unroll
-    for (int k = 0; k < kQuant; k++) {
-        const int64_t i = i0 + 256 * k;
-        if (i < total) {  // the four lanes of a block are in or out together
-            const float *p = x + (unit ? (i / unit) * ldx + (i % unit) * 8 : i * 8);
-            const Float4 a = *reinterpret_cast<const Float4 *>(p), b = *reinterpret_cast<const Float4 *>(p + 4);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[k][j] = a.x[j];
-                v[k][4 + j] = b.x[j];
-            }
-        }
+    for (int k = 0; k < 2 * kQuant; k++) {
+        const int64_t i = i0 + 64 * k;
+        if (i < total) v[k] = *reinterpret_cast<const Float4 *>(x + (unit ? (i / unit) * ldx + (i % unit) * 4 : i * 4));
     }
+    const bool odd = threadIdx.x & 1;
 #pragma unroll
     for (int k = 0; k < kQuant; k++) {
-        const int64_t i = i0 + 256 * k;
-        if (i < total) {
-            int e;
-            codes[i] = quant_quarter(v[k], &e);
-            if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)e;
+        uint32_t word[2];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const float *y = v[2 * k + s].x;
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
+            m = quad_max(m);
+            m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));  // row_half_mirror
+            const int e = scale_of_bits(m);
+            const float inv = inverse_scale(e);
+            uint32_t c = 0;
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[0] * inv, y[1] * inv, 1.0f, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2] * inv, y[3] * inv, 1.0f, 1);
+            if (e == 255) c = 0;
+            const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0xB1, 0xF, 0xF, false);
+            word[s] = odd ? other | c << 16 : c | other << 16;
+            const int64_t i = i0 + 64 * (2 * k + s);  // the eight lanes of a block are in or out together
+            if ((threadIdx.x & 7) == 0 && i < total) scales[i >> 3] = (uint8_t)e;
         }
+        const int64_t i = i0 + 64 * (2 * k + (odd ? 1 : 0));
+        if (i < total) codes[i >> 1] = odd ? word[1] : word[0];
     }
 }
 
@@ -526,23 +538,24 @@ int check_codes(const char *name, const llmq_ctx *ctx, const void *a, const void
     return LLMQ_OK;
 }
 
-// The quarter-block kernels' grid, and lanes a row (0: the rows lie together).
-struct Quarters {
+// The grid of a kernel whose workgroups take `each` pieces of `values` values, and pieces a row (0: the rows
+// lie together).
+struct Pieces {
     int64_t total, grid;
     uint32_t unit;
 };
-int quarters(const char *name, int64_t T, int64_t K, int64_t ld, Quarters *out) {
-    out->total = T * (K / 8);
-    out->grid = (out->total + 256 * kQuant - 1) / (256 * kQuant);
-    out->unit = ld == K || T == 1 ? 0 : (uint32_t)(K / 8);
+int pieces(const char *name, int64_t T, int64_t K, int64_t ld, int values, int each, Pieces *out) {
+    out->total = T * (K / values);
+    out->grid = (out->total + each - 1) / each;
+    out->unit = ld == K || T == 1 ? 0 : (uint32_t)(K / values);
     LLMQ_REQUIRE(out->grid <= INT32_MAX, "%s: %lld rows of %lld", name, (long long)T, (long long)K);
     return LLMQ_OK;
 }
 
 int launch_quantize(llmq_ctx *ctx, const float *x, int64_t ldx, int64_t T, int64_t K, uint8_t *codes,
                     uint8_t *scales) {
-    Quarters u;
-    RC(quarters("mx4_quantize", T, K, ldx, &u));
+    Pieces u;
+    RC(pieces("mx4_quantize", T, K, ldx, 4, 256 * 2 * kQuant, &u));
     hipLaunchKernelGGL(mx4_quantize_kernel, dim3((unsigned)u.grid), dim3(256), 0, ctx->stream, x, ldx, u.unit, u.total,
                        reinterpret_cast<uint32_t *>(codes), scales);
     LLMQ_HIP(hipGetLastError());
@@ -673,8 +686,8 @@ int llmq_mx4_dequantize(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scal
     LLMQ_REQUIRE(ldo >= K, "mx4_dequantize: rows of %lld floats %lld apart", (long long)K, (long long)ldo);
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
-    Quarters u;
-    RC(quarters("mx4_dequantize", T, K, ldo, &u));
+    Pieces u;
+    RC(pieces("mx4_dequantize", T, K, ldo, 8, 256 * kQuant, &u));
     hipLaunchKernelGGL(mx4_dequantize_kernel, dim3((unsigned)u.grid), dim3(256), 0, ctx->stream,
                        reinterpret_cast<const uint32_t *>(codes), scales, u.unit, u.total, out, ldo);
     LLMQ_HIP(hipGetLastError());

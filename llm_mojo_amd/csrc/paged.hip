@@ -143,6 +143,32 @@ __device__ __forceinline__ Dest dest_of(const Layer &c, const int32_t *seq, cons
     return d;
 }
 
+// The rows of workgroup i: from the first row of its kRows that begins a
+// block or does not follow the row before, to the next workgroup's first such.
+// So a block whose positions are neighbouring rows is one workgroup's, which
+// writes its lines whole, wherever the rows begin.  At most 2 kRows - 1 of
+// them: neighbouring rows begin a block every kRows.
+struct Span {
+    int64_t lo, hi;
+};
+__device__ __forceinline__ Span rows_of(const int32_t *seq, const int32_t *pos, int64_t i, int64_t T, int lane) {
+    static_assert(kRows == B, "a workgroup's rows and a block's");
+    const int64_t t = i * kRows + lane;
+    bool first = false;
+    if (t < T) {
+        const int p = pos[t];
+        first = t == 0 || p % B == 0 || seq[t - 1] != seq[t] || (uint32_t)pos[t - 1] + 1u != (uint32_t)p;
+    }
+    const uint64_t all = __ballot(first);
+    const uint32_t here = (uint32_t)all, next = (uint32_t)(all >> 32);
+    const int64_t end = (i + 1) * kRows;
+    Span s;
+    s.hi = next ? end + __ffs(next) - 1 : (end + kRows < T ? end + kRows : T);
+    s.lo = here ? i * kRows + __ffs(here) - 1 : s.hi;
+    if (s.hi > T) s.hi = T;
+    return s;
+}
+
 // Maximum over the eight lanes of a row.
 __device__ __forceinline__ float eighth_max(float v) {
     v = fmaxf(v, llmq_dppf<0xB1>(v));
@@ -164,59 +190,63 @@ __global__ __launch_bounds__(kRows *kLanes) void pkv_store_kernel(Layer c, const
     __shared__ __align__(4) uint8_t vt[kRows * STRIDE];
     __shared__ int64_t at[kRows];
     const int tid = threadIdx.x, row = tid / kLanes, j = tid % kLanes, head = blockIdx.y;
-    const int64_t t = (int64_t)blockIdx.x * kRows + row;
-    const Dest d = dest_of<HD>(c, seq, pos, n_seq, t, T, head);
-    if (j == 0) at[row] = d.value;
-    if (d.row >= 0) {
-        const float *src[2] = {k + t * ld + head * HD, v + t * ld + head * HD};
-        float x[2][NP][4];
+    const Span span = rows_of(seq, pos, blockIdx.x, T, tid & 63);
+    for (int64_t begin = span.lo; begin < span.hi; begin += kRows) {
+        if (begin > span.lo) __syncthreads();  // the rows before are through
+        const int64_t t = begin + row;
+        const Dest d = dest_of<HD>(c, seq, pos, n_seq, t, span.hi, head);
+        if (j == 0) at[row] = d.value;
+        if (d.row >= 0) {
+            const float *src[2] = {k + t * ld + head * HD, v + t * ld + head * HD};
+            float x[2][NP][4];
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int i = 0; i < NP; i++)
-                *reinterpret_cast<Floats4 *>(x[s][i]) = *reinterpret_cast<const Floats4 *>(src[s] + 32 * i + 4 * j);
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            uint8_t *keys = s == 0 ? c.k + d.row * HD * ELEM : vt + row * STRIDE;
-            if constexpr (ELEM == 1) {
-                float m = 0.0f, bad = 0.0f;
+            for (int s = 0; s < 2; s++)
 #pragma unroll
                 for (int i = 0; i < NP; i++)
+                    *reinterpret_cast<Floats4 *>(x[s][i]) = *reinterpret_cast<const Floats4 *>(src[s] + 32 * i + 4 * j);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        m = fmaxf(m, fabsf(x[s][i][e]));
-                        bad += x[s][i][e] - x[s][i][e];  // NaN for NaN and infinities
+            for (int s = 0; s < 2; s++) {
+                uint8_t *keys = s == 0 ? c.k + d.row * HD * ELEM : vt + row * STRIDE;
+                if constexpr (ELEM == 1) {
+                    float m = 0.0f, bad = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NP; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            m = fmaxf(m, fabsf(x[s][i][e]));
+                            bad += x[s][i][e] - x[s][i][e];  // NaN for NaN and infinities
+                        }
+                    m = eighth_max(bad != 0.0f || bad != bad ? INFINITY : m);
+                    const float scale = row_scale(m), inv = 1.0f / scale;
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        uint32_t u = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) u |= (uint32_t)row_code(x[s][i][e], inv) << (8 * e);
+                        *reinterpret_cast<uint32_t *>(keys + 32 * i + 4 * j) = u;
                     }
-                m = eighth_max(bad != 0.0f || bad != bad ? INFINITY : m);
-                const float scale = row_scale(m), inv = 1.0f / scale;
+                    if (j == 0) (s == 0 ? c.ks : c.vs)[d.row] = scale;
+                } else {
 #pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    uint32_t u = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) u |= (uint32_t)row_code(x[s][i][e], inv) << (8 * e);
-                    *reinterpret_cast<uint32_t *>(keys + 32 * i + 4 * j) = u;
-                }
-                if (j == 0) (s == 0 ? c.ks : c.vs)[d.row] = scale;
-            } else {
-#pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    uint32_t *u = reinterpret_cast<uint32_t *>(keys + 64 * i + 8 * j);
-                    u[0] = half_bits(x[s][i][0]) | (uint32_t)half_bits(x[s][i][1]) << 16;
-                    u[1] = half_bits(x[s][i][2]) | (uint32_t)half_bits(x[s][i][3]) << 16;
+                    for (int i = 0; i < NP; i++) {
+                        uint32_t *u = reinterpret_cast<uint32_t *>(keys + 64 * i + 8 * j);
+                        u[0] = half_bits(x[s][i][0]) | (uint32_t)half_bits(x[s][i][1]) << 16;
+                        u[1] = half_bits(x[s][i][2]) | (uint32_t)half_bits(x[s][i][3]) << 16;
+                    }
                 }
             }
         }
-    }
-    __syncthreads();
+        __syncthreads();
 #pragma unroll 4
-    for (int i = tid; i < kRows * HD; i += kRows * kLanes) {
-        const int e = i % kRows, dim = i / kRows;
-        if (at[e] < 0) continue;
-        if constexpr (ELEM == 1)
-            c.v[at[e] + dim * B] = vt[e * STRIDE + dim];
-        else
-            reinterpret_cast<uint16_t *>(c.v)[at[e] + dim * B] =
-                *reinterpret_cast<const uint16_t *>(vt + e * STRIDE + 2 * dim);
+        for (int i = tid; i < kRows * HD; i += kRows * kLanes) {
+            const int e = i % kRows, dim = i / kRows;
+            if (at[e] < 0) continue;
+            if constexpr (ELEM == 1)
+                c.v[at[e] + dim * B] = vt[e * STRIDE + dim];
+            else
+                reinterpret_cast<uint16_t *>(c.v)[at[e] + dim * B] =
+                    *reinterpret_cast<const uint16_t *>(vt + e * STRIDE + 2 * dim);
+        }
     }
 }
 
@@ -230,53 +260,57 @@ __global__ __launch_bounds__(kRows *kLanes) void pkv_fetch_kernel(Layer c, float
     __shared__ __align__(4) uint8_t vt[kRows * STRIDE];
     __shared__ int64_t at[kRows];
     const int tid = threadIdx.x, row = tid / kLanes, j = tid % kLanes, head = blockIdx.y;
-    const int64_t t = (int64_t)blockIdx.x * kRows + row;
-    const Dest d = dest_of<HD>(c, seq, pos, n_seq, t, T, head);
-    if (j == 0) at[row] = d.value;
-    uint32_t key[NP][ELEM];
-    float ks = 1.0f, vs = 1.0f;
-    if (d.row >= 0) {
+    const Span span = rows_of(seq, pos, blockIdx.x, T, tid & 63);
+    for (int64_t begin = span.lo; begin < span.hi; begin += kRows) {
+        if (begin > span.lo) __syncthreads();  // the rows before are through
+        const int64_t t = begin + row;
+        const Dest d = dest_of<HD>(c, seq, pos, n_seq, t, span.hi, head);
+        if (j == 0) at[row] = d.value;
+        uint32_t key[NP][ELEM];
+        float ks = 1.0f, vs = 1.0f;
+        if (d.row >= 0) {
 #pragma unroll
-        for (int i = 0; i < NP; i++)
+            for (int i = 0; i < NP; i++)
 #pragma unroll
-            for (int e = 0; e < ELEM; e++)
-                key[i][e] = *reinterpret_cast<const uint32_t *>(c.k + (d.row * HD + 32 * i + 4 * j) * ELEM + 4 * e);
-        if constexpr (ELEM == 1) {
-            ks = c.ks[d.row];
-            vs = c.vs[d.row];
-        }
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int i = tid; i < kRows * HD; i += kRows * kLanes) {
-        const int e = i % kRows, dim = i / kRows;
-        if (at[e] < 0) continue;
-        if constexpr (ELEM == 1)
-            vt[e * STRIDE + dim] = c.v[at[e] + dim * B];
-        else
-            *reinterpret_cast<uint16_t *>(vt + e * STRIDE + 2 * dim) =
-                reinterpret_cast<const uint16_t *>(c.v)[at[e] + dim * B];
-    }
-    __syncthreads();
-    if (t >= T) return;
-#pragma unroll
-    for (int i = 0; i < NP; i++) {
-        Floats4 x{}, y{};
-        if (d.row >= 0)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int dim = 32 * i + 4 * j + e;
-                if constexpr (ELEM == 1) {
-                    x.x[e] = (float)((int)((key[i][0] >> (8 * e)) & 255) - kBias) * ks;
-                    y.x[e] = (float)((int)vt[row * STRIDE + dim] - kBias) * vs;
-                } else {
-                    x.x[e] = __half2float(__ushort_as_half((uint16_t)(key[i][e >> 1] >> (16 * (e & 1)))));
-                    y.x[e] = __half2float(
-                        __ushort_as_half(*reinterpret_cast<const uint16_t *>(vt + row * STRIDE + 2 * dim)));
-                }
+                for (int e = 0; e < ELEM; e++)
+                    key[i][e] = *reinterpret_cast<const uint32_t *>(c.k + (d.row * HD + 32 * i + 4 * j) * ELEM + 4 * e);
+            if constexpr (ELEM == 1) {
+                ks = c.ks[d.row];
+                vs = c.vs[d.row];
             }
-        *reinterpret_cast<Floats4 *>(k + t * ld + head * HD + 32 * i + 4 * j) = x;
-        *reinterpret_cast<Floats4 *>(v + t * ld + head * HD + 32 * i + 4 * j) = y;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid; i < kRows * HD; i += kRows * kLanes) {
+            const int e = i % kRows, dim = i / kRows;
+            if (at[e] < 0) continue;
+            if constexpr (ELEM == 1)
+                vt[e * STRIDE + dim] = c.v[at[e] + dim * B];
+            else
+                *reinterpret_cast<uint16_t *>(vt + e * STRIDE + 2 * dim) =
+                    reinterpret_cast<const uint16_t *>(c.v)[at[e] + dim * B];
+        }
+        __syncthreads();
+        if (t >= span.hi) continue;
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            Floats4 x{}, y{};
+            if (d.row >= 0)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int dim = 32 * i + 4 * j + e;
+                    if constexpr (ELEM == 1) {
+                        x.x[e] = (float)((int)((key[i][0] >> (8 * e)) & 255) - kBias) * ks;
+                        y.x[e] = (float)((int)vt[row * STRIDE + dim] - kBias) * vs;
+                    } else {
+                        x.x[e] = __half2float(__ushort_as_half((uint16_t)(key[i][e >> 1] >> (16 * (e & 1)))));
+                        y.x[e] = __half2float(
+                            __ushort_as_half(*reinterpret_cast<const uint16_t *>(vt + row * STRIDE + 2 * dim)));
+                    }
+                }
+            *reinterpret_cast<Floats4 *>(k + t * ld + head * HD + 32 * i + 4 * j) = x;
+            *reinterpret_cast<Floats4 *>(v + t * ld + head * HD + 32 * i + 4 * j) = y;
+        }
     }
 }
 
@@ -810,10 +844,11 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
 constexpr int kJoinWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Attend a) {
-    __shared__ float wl[kJoinWaves], ws[kJoinWaves][HD];
+    __shared__ float2 wl[kJoinWaves];
+    __shared__ float ws[kJoinWaves][HD];
     const int64_t r = blockIdx.y;
     const int h = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int2 m = a.meta[r];
+    const int2 m = a.meta[r];
     if (row_len(c, a, r) == 0) {  // in no slot
         if (threadIdx.x < HD) a.out[r * a.ldo + (int64_t)h * HD + threadIdx.x] = 0.0f;
         return;
@@ -821,26 +856,57 @@ __global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Atte
     if (m.x == m.y) return;  // in one, which has written it
     const float2 *ml = a.ml + (int64_t)m.x * a.n_head + h;
     const float *sums = a.sums + ((int64_t)m.x * a.n_head + h) * HD;
-    m.y = m.y - m.x + 1;
-    float R = kLowest;
-    for (int i = lane; i < m.y; i += 64) R = fmaxf(R, ml[(int64_t)i * a.n_head].x);
-    R = llmq_wave_max_all(R);
-    float L = 0.0f, o[HD / 64] = {};
-#pragma unroll 4
-    for (int i = w; i < m.y; i += kJoinWaves) {
-        const float2 x = ml[(int64_t)i * a.n_head];
-        const float f = exp2f(x.x - R);
-        L = fmaf(x.y, f, L);
+    const int n = m.y - m.x + 1;
+    // a wave every fourth segment, kAtOnce of them asked for together
+    constexpr int kAtOnce = 8;
+    float R = kLowest, L = 0.0f, o[HD / 64] = {};
+    for (int i0 = w; i0 < n; i0 += kJoinWaves * kAtOnce) {
+        float2 x[kAtOnce];
+        float s[kAtOnce][HD / 64];
 #pragma unroll
-        for (int d = 0; d < HD / 64; d++) o[d] = fmaf(sums[(int64_t)i * a.n_head * HD + lane + 64 * d], f, o[d]);
+        for (int k = 0; k < kAtOnce; k++) {
+            const int i = i0 + kJoinWaves * k;
+            x[k] = make_float2(kLowest, 0.0f);
+            if (i < n) {
+                x[k] = ml[(int64_t)i * a.n_head];
+#pragma unroll
+                for (int d = 0; d < HD / 64; d++) s[k][d] = sums[(int64_t)i * a.n_head * HD + lane + 64 * d];
+            } else {
+#pragma unroll
+                for (int d = 0; d < HD / 64; d++) s[k][d] = 0.0f;
+            }
+        }
+        float to = R;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) to = fmaxf(to, x[k].x);
+        const float f = exp2f(R - to);
+        R = to;
+        L *= f;
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) o[d] *= f;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const float g = exp2f(x[k].x - R);
+            L = fmaf(x[k].y, g, L);
+#pragma unroll
+            for (int d = 0; d < HD / 64; d++) o[d] = fmaf(s[k][d], g, o[d]);
+        }
     }
-    if (lane == 0) wl[w] = L;
+    if (lane == 0) wl[w] = make_float2(R, L);
 #pragma unroll
     for (int d = 0; d < HD / 64; d++) ws[w][lane + 64 * d] = o[d];
     __syncthreads();
     if (threadIdx.x < HD) {
         const int d = threadIdx.x;
-        const float all = (wl[0] + wl[1]) + (wl[2] + wl[3]), s = (ws[0][d] + ws[1][d]) + (ws[2][d] + ws[3][d]);
+        float to = kLowest, all = 0.0f, s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoinWaves; k++) to = fmaxf(to, wl[k].x);
+#pragma unroll
+        for (int k = 0; k < kJoinWaves; k++) {
+            const float g = exp2f(wl[k].x - to);
+            all = fmaf(wl[k].y, g, all);
+            s = fmaf(ws[k][d], g, s);
+        }
         a.out[r * a.ldo + (int64_t)h * HD + d] = all == 0.0f ? 0.0f : s / all;
     }
 }

@@ -158,6 +158,45 @@ def test_store_and_fetch(gpu, kind, hd):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_store_runs_of_rows(gpu, kind):
+    """Rows in order (as prompts come), of sequences that begin and end
+    anywhere: runs from one row to several blocks, at every offset in a block,
+    with padding rows and jumps between them."""
+    torch, lm, ctx = gpu
+    rng = np.random.default_rng(11)
+    for trial in range(6):
+        n_seq, width, page = 7, 5, 64
+        table = rng.permutation(n_seq * width + 2)[:n_seq * width].astype(np.int32).reshape(n_seq, width)
+        cache = lm.PagedKV(ctx, 1, n_seq * width + 2, page, 2, 64, kind)
+        seq, pos = [], []
+        for s in range(n_seq):
+            at = int(rng.integers(0, 70))
+            while at < width * page:
+                n = int(rng.choice([1, 2, 31, 32, 33, 64, 100]))
+                run = list(range(at, min(at + n, width * page)))
+                seq += [s] * len(run)
+                pos += run
+                at = run[-1] + 1 + int(rng.choice([0, 0, 1, 40]))
+                if rng.random() < 0.3:
+                    pad = int(rng.integers(1, 40))
+                    seq += [-1] * pad
+                    pos += list(range(pad))
+        seq, pos = np.array(seq, np.int32), np.array(pos, np.int32)
+        k, v = (rng.normal(0, 1, (len(seq), 2, 64)).astype(np.float32) for _ in range(2))
+        d = lambda a: dev(torch, a)  # noqa: E731
+        cache.store(0, d(k), d(v), d(seq), d(pos), d(table))
+        ko, vo = (torch.full(k.shape, float("nan"), device="cuda") for _ in range(2))
+        cache.fetch(0, ko, vo, d(seq), d(pos), d(table))
+        live = (seq >= 0)[:, None, None]
+        assert np.array_equal(ko.cpu().numpy(), np.where(live, held(kind, k), 0))
+        assert np.array_equal(vo.cpu().numpy(), np.where(live, held(kind, v), 0))
+        # and one row at a time
+        back = rng.permutation(len(seq))
+        cache.fetch(0, ko, vo, d(seq[back]), d(pos[back]), d(table))
+        assert np.array_equal(ko.cpu().numpy(), np.where(live, held(kind, k), 0)[back])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_store_leaves_out_and_overwrites_nothing_else(gpu, kind):
     """Padding rows, positions past the table, pages that are none: nothing is
     written; fetch gives zeros for them."""
