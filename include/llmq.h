@@ -173,8 +173,8 @@ LLMQ_API int llmq_dot_row_i16(llmq_ctx *ctx, const llmq_mat *mat, int64_t row, i
  * memory (outputs by inputs), which llmq_mat_export_mx4 gives back (either
  * may be NULL there).  Both operands of its products are microscaled:
  * llmq_linear, llmq_linear_noalloc and llmq_head quantize their rows of x as
- * above and then multiply (scratch of llmq_linear_noalloc: T x IN x 17 / 32
- * bytes and up to 256); under graph capture llmq_linear refuses several
+ * above and then multiply (scratch of llmq_linear_noalloc: 17 / 32 bytes a
+ * value, T rounded up to 16 and IN to 512); under graph capture llmq_linear refuses several
  * tokens (its workspace is the context's): quantize into memory of your own
  * and call llmq_mx4_linear. */
 LLMQ_API int llmq_mat_from_f32_mx4(llmq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int reduce_rows,

@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "common.h"
@@ -145,6 +146,43 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const float *__restri
     }
 }
 
+// The same into a record: tokens in tiles of 16 laid out as a matrix's rows
+// are, so that a product's operand is 1 KB in one piece (rows of packed codes
+// 2 KB apart, at 4096 inputs, meet in few of L2's channels: 2048 x 4096 x
+// 11008 took 71 us from those and 61 from a record).  A workgroup 16 tokens and
+// a group of four steps, a wave a block of each step; tokens and blocks past
+// the end become zeros with scale 127.
+__global__ __launch_bounds__(256) void mx4_record_kernel(const float *__restrict__ x, int64_t T, int nb, int words,
+                                                         uint32_t *__restrict__ codes, uint32_t *__restrict__ scales) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = lane >> 2, quarter = lane & 3, g = blockIdx.x;
+    const int64_t tile = blockIdx.y, t = tile * 16 + row;
+    float v[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int b = g * 16 + 4 * j + w;
+        if (t < T && b < nb) {
+            const float *p = x + (t * nb + b) * 32 + quarter * 8;
+            const Float4 y = *reinterpret_cast<const Float4 *>(p), z = *reinterpret_cast<const Float4 *>(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[j][i] = y.x[i];
+                v[j][4 + i] = z.x[i];
+            }
+        }
+    }
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int b = g * 16 + 4 * j + w;
+        int e = 127;
+        uint32_t code = 0;
+        if (t < T && b < nb) code = quant_quarter(v[j], &e);  // four lanes of a block: in or out together
+        word |= (uint32_t)e << (8 * j);
+        codes[(((tile * words + g) * 4 + j) * 64 + row + 16 * w) * 4 + quarter] = code;
+    }
+    if (quarter == 0) scales[(tile * words + g) * 64 + row + 16 * w] = word;
+}
+
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ scales, uint32_t unit,
                                                              int64_t total, float *__restrict__ out, int64_t ldo) {
@@ -202,8 +240,9 @@ __device__ __forceinline__ void finish(float *p, float y, const float *bias, int
     *p = y;
 }
 
-// Operands of a product: tokens quantized in rows (codes K / 2 and scales
-// K / 32 bytes each; nb blocks), the matrix in its layout.
+// Operands of a product: tokens in packed rows (codes K / 2 and scales K / 32
+// bytes each; nb blocks) or a record, the matrix in its layout.
+enum { kRows = 0, kRecord = 1, kFloats = 2 };  // how a kernel is given its tokens (kFloats: one)
 struct Product {
     const uint8_t *xc, *xs;
     const uint8_t *wc;
@@ -233,13 +272,12 @@ __device__ __forceinline__ v4f mma(const uint4 &a, const uint4 &b, const v4f &c,
 struct Bytes16 {
     uint32_t x[4];
 } __attribute__((packed, aligned(1)));
-__device__ __forceinline__ uint32_t token_scales(const uint8_t *row, int nb, int g, int q) {
-    if (g * 16 + 16 <= nb) {
-        const Bytes16 s = *reinterpret_cast<const Bytes16 *>(row + g * 16);
-        const uint32_t sel = 0x0400u + 0x0101u * q;
-        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(s.x[3], s.x[2], sel),
-                                     __builtin_amdgcn_perm(s.x[1], s.x[0], sel), 0x05040100u);
-    }
+__device__ __forceinline__ uint32_t pack_scales(const Bytes16 &s, int q) {
+    const uint32_t sel = 0x0400u + 0x0101u * q;
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(s.x[3], s.x[2], sel),
+                                 __builtin_amdgcn_perm(s.x[1], s.x[0], sel), 0x05040100u);
+}
+__device__ __forceinline__ uint32_t tail_scales(const uint8_t *row, int nb, int g, int q) {
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -248,17 +286,26 @@ __device__ __forceinline__ uint32_t token_scales(const uint8_t *row, int nb, int
     }
     return w;
 }
+__device__ __forceinline__ uint32_t token_scales(const uint8_t *row, int nb, int g, int q) {
+    if (g * 16 + 16 > nb) return tail_scales(row, nb, g, q);
+    return pack_scales(*reinterpret_cast<const Bytes16 *>(row + g * 16), q);
+}
 
 // Waves of a few-token workgroup at most: with four token tiles its registers hold half as many.
 constexpr int few_most(int tt) { return tt < 4 ? 16 : 8; }
 
 // Few tokens: a workgroup 16 outputs and TT tiles of 16 tokens, its waves
-// taking whole groups of four steps in turn (`per` each), their sums added in
-// LDS in wave order.  Bound by the weights, read once a TT tiles; all of a
-// group's operands are asked for before the first product.  FUSED: one token
-// from its floats, quantized by every workgroup into LDS while its weights
-// are on their way, in place of a launch that writes 17 / 32 K bytes.
-template <int TT, bool FUSED>
+// taking groups of four steps (`per` each, in a row), their sums added in LDS
+// in wave order: the matrix's few tiles become many waves with all of a
+// group's operands asked for before its first product, and the next group's
+// weights.  Bound by the weights for one token tile, then by the tokens'
+// codes, which every workgroup reads (two tiles of outputs a workgroup halve
+// that and were slower at every size measured: 64 x 4096 x 11008 14.9 us
+// against 11.3).  kFloats: one token from its floats, quantized by every
+// workgroup into LDS while its weights are on their way, in place of a launch
+// that writes 17 / 32 K bytes.  4096 x 11008 for one token 5.4-6.3 us, the
+// read of its 24 MB alone 5.6.
+template <int TT, int X>
 __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, int per) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4,
@@ -270,11 +317,14 @@ __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, i
     const int rowb = p.nb * 16;
     const int64_t left = p.T - t0;
     const int live = (int)(left < 16 * TT ? left : 16 * TT);
-    const auto rx = llmq_rsrc(FUSED ? p.wc : p.xc + t0 * rowb, FUSED ? 0 : (uint32_t)live * rowb);
-    uint8_t *fs = lds, *fc = lds + p.words * 16;  // FUSED: scales [group][q][step], codes
+    const uint32_t tiles = (uint32_t)(live + 15) / 16;
+    const auto rx = X == kRows     ? llmq_rsrc(p.xc + t0 * rowb, (uint32_t)live * rowb)
+                    : X == kRecord ? llmq_rsrc(p.xc + t0 / 16 * p.words * 4096, tiles * p.words * 4096)
+                                   : llmq_rsrc(p.wc, 0);
+    uint8_t *fs = lds, *fc = lds + p.words * 16;  // kFloats: scales [group][q][step], codes
 
     uint4 a[4];
-    uint32_t as = 0;
+    uint32_t as;
     auto weights = [&](int g) {
 #pragma unroll
         for (int j = 0; j < 4; j++)  // zeros past the last step, without reading them
@@ -284,7 +334,7 @@ __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, i
     int g = w * per;
     const int end = min(g + per, p.words);
     if (g < end) weights(g);
-    if constexpr (FUSED) {
+    if constexpr (X == kFloats) {
         const int units = p.words * 64;  // quarters of blocks
         for (int i = tid; i < units; i += blockDim.x) {
             float v[8];
@@ -314,10 +364,15 @@ __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, i
         uint32_t bs[TT];
 #pragma unroll
         for (int t = 0; t < TT; t++) {
-            if constexpr (FUSED) {  // the token in every column
+            if constexpr (X == kFloats) {  // the token in every column
                 bs[t] = *reinterpret_cast<const uint32_t *>(fs + g * 16 + q * 4);
 #pragma unroll
                 for (int j = 0; j < 4; j++) b[t][j] = *reinterpret_cast<const uint4 *>(fc + (g * 4 + j) * 64 + q * 16);
+            } else if constexpr (X == kRecord) {
+                const int64_t at = t0 / 16 + min(t, (live - 1) / 16);
+                bs[t] = reinterpret_cast<const uint32_t *>(p.xs)[(at * p.words + g) * 64 + lane];
+#pragma unroll
+                for (int j = 0; j < 4; j++) b[t][j] = llmq_bload16(rx, ((t * p.words + g) * 4 + j) * 1024 + lane * 16);
             } else {
                 const int row = min(16 * t + c, live - 1);
                 bs[t] = token_scales(p.xs + (t0 + row) * p.nb, p.nb, g, q);
@@ -337,11 +392,10 @@ __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, i
     }
     // [wave][tile][token][output]
     float *sum = reinterpret_cast<float *>(lds);
-    if constexpr (FUSED) __syncthreads();
+    if constexpr (X == kFloats) __syncthreads();
 #pragma unroll
     for (int t = 0; t < TT; t++)
-        if (!FUSED || c == 0)
-            *reinterpret_cast<v4f *>(sum + ((w * TT + t) * 16 + c) * 16 + 4 * q) = acc[t];
+        if (X != kFloats || c == 0) *reinterpret_cast<v4f *>(sum + ((w * TT + t) * 16 + c) * 16 + 4 * q) = acc[t];
     __syncthreads();
     for (int i = tid; i < live * 16; i += blockDim.x) {
         const int o = tile * 16 + (i & 15);
@@ -351,18 +405,23 @@ __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, i
     }
 }
 
-// Many tokens: a workgroup 256 outputs and 128 tokens, a wave 64 of the
-// outputs by all the tokens (32 accumulators).  The tokens' codes are shared
-// by the four waves: they are copied to LDS a group of four steps ahead, each
-// fragment as the 1 KB that a wave reads of it, without passing through
-// registers; their scales are put into words there a group ahead.  A wave's
-// weights, which no other wave of the workgroup reads, come straight to its
-// registers two steps ahead, 1 KB in one piece.  A step is 32 products of 16
-// cycles to 8 KB of LDS reads a wave: half of what LDS gives.
-constexpr int kTokens = 128, kOuts = 256;
+// Many tokens: a workgroup 256 outputs and TT tiles of 16 tokens, a wave 64 of
+// the outputs by all the tokens.  The tokens' codes are shared by the four
+// waves: they are copied to LDS a group of four steps ahead, each fragment as
+// the 1 KB that a wave reads of it, without passing through registers; their
+// scales are put into words there a group ahead.  A wave's weights, which no
+// other wave of the workgroup reads, come straight to its registers three
+// steps ahead, 1 KB in one piece.  With the loads, copies, barriers and LDS
+// reads left out, 2048 x 4096 x 11008 still takes 38 us of the 58 that the
+// kernel takes: 18 of products (16 cycles each), the rest its 90 MB of outputs.  Tiles
+// of 128 tokens need more than 256 registers.
+constexpr int kOuts = 256;
+template <int TT, int X>
 __global__ __launch_bounds__(256, 2) void mx4_many_kernel(Product p, int gx, int gy) {
-    __shared__ __align__(16) uint8_t c0[32768], c1[32768];
-    __shared__ uint32_t s0[512], s1[512];
+    constexpr int kTokens = 16 * TT;
+    __shared__ __align__(16) uint8_t c0[TT * 4096], c1[TT * 4096];
+    constexpr int NS = (TT + 3) / 4;  // words of the tokens' scales a thread
+    __shared__ uint32_t s0[NS * 256], s1[NS * 256];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4,
               c = lane & 15;
     // an XCD takes neighbouring tiles, the tokens' fastest: it reads its part of the weights once
@@ -373,7 +432,9 @@ __global__ __launch_bounds__(256, 2) void mx4_many_kernel(Product p, int gx, int
     const int rowb = p.nb * 16;
     const int64_t left = p.T - t0;
     const int live = (int)(left < kTokens ? left : kTokens);
-    const auto rx = llmq_rsrc(p.xc + t0 * rowb, (uint32_t)live * rowb);
+    const uint32_t tiles = (uint32_t)(live + 15) / 16;
+    const auto rx = X == kRows ? llmq_rsrc(p.xc + t0 * rowb, (uint32_t)live * rowb)
+                               : llmq_rsrc(p.xc + t0 / 16 * p.words * 4096, tiles * p.words * 4096);
     const int tile0 = bo * 16 + w * 4;
     int so[4];  // the wave's row tiles (its first again past the matrix's end)
     const int base = min(tile0, p.ntiles - 1);
@@ -384,30 +445,54 @@ __global__ __launch_bounds__(256, 2) void mx4_many_kernel(Product p, int gx, int
     const uint32_t *ws = p.ws + (int64_t)base * p.words * 64 + lane;
     const int groups = p.words;
 
-    auto stage = [&](int g, uint8_t *dst) __attribute__((always_inline)) {
+    auto stage = [&](int g, uint8_t *dst) __attribute__((always_inline)) {  // wave w: step w of the group
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int t = 2 * w + i;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    rx, (__attribute__((address_space(3))) void *)(dst + (j * 8 + t) * 1024), 16,
-                    (16 * t + c) * rowb + q * 16 + (g * 4 + j) * 64, 0, 0, 0);
-            }
+        for (int t = 0; t < TT; t++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rx, (__attribute__((address_space(3))) void *)(dst + (w * TT + t) * 1024), 16,
+                X == kRows ? (16 * t + c) * rowb + q * 16 + (g * 4 + w) * 64
+                           : ((t * p.words + g) * 4 + w) * 1024 + lane * 16,
+                0, 0, 0);
     };
-    auto scales = [&](int g, uint32_t *dst) __attribute__((always_inline)) {
+    // the thread's tokens' scales: asked for at a group's start, put into words at its end
+    const uint8_t *xs[NS];
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = tid + 256 * k, row = min(i >> 6 << 4 | (i & 15), live - 1);
-            dst[i] = token_scales(p.xs + (t0 + row) * p.nb, p.nb, g, (i >> 4) & 3);
+    for (int k = 0; k < NS; k++) {
+        if constexpr (X == kRows)
+            xs[k] = p.xs + (t0 + min((w + 4 * k) * 16 + c, live - 1)) * p.nb;
+        else
+            xs[k] = p.xs + ((t0 / 16 + min(w + 4 * k, (live - 1) / 16)) * p.words * 64 + lane) * 4;
+    }
+    uint32_t raw[NS][4];
+    auto ask = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            if constexpr (X == kRecord) {
+                raw[k][0] = *reinterpret_cast<const uint32_t *>(xs[k] + (int64_t)g * 256);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) raw[k][j] = xs[k][min(g * 16 + 4 * j + q, p.nb - 1)];
+            }
         }
     };
-    v4f acc[4][8];
+    auto put = [&](int g, uint32_t *dst) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            uint32_t word = raw[k][0];
+            if constexpr (X == kRows) {  // 127 past the row's end, as in tail_scales
+                word = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) word |= (g * 16 + 4 * j + q < p.nb ? raw[k][j] : 127u) << (8 * j);
+            }
+            dst[tid + 256 * k] = word;
+        }
+    };
+    v4f acc[4][TT];
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int t = 0; t < 8; t++) acc[r][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    uint4 a[3][4];
+        for (int t = 0; t < TT; t++) acc[r][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    uint4 a[4][4];
     auto weights = [&](int s, uint4 (&dst)[4]) __attribute__((always_inline)) {
         const int k = min(s, 4 * p.words - 1);  // (past the end: loaded and not used)
 #pragma unroll
@@ -420,50 +505,65 @@ __global__ __launch_bounds__(256, 2) void mx4_many_kernel(Product p, int gx, int
 #pragma unroll
     for (int r = 0; r < 4; r++) as[r] = ws[so[r] * p.words * 64];
     stage(0, c0);
-    scales(0, s0);
-    weights(0, a[0]);
-    weights(1, a[1]);
+    ask(0);
+    put(0, s0);
+#pragma unroll
+    for (int s = 0; s < 3; s++) weights(s, a[s]);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the first group's copies, which fewer loads follow
     auto group = [&](int g, const uint8_t *cb, uint8_t *nb, const uint32_t *sb, uint32_t *ns)
         __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this wave's copies are in, its reads done
+        // vmcnt(16), lgkmcnt(0): this wave's copies are in, behind which it has asked for the weights of the last
+        // group's four steps only (4 loads each), and its reads are done
+        __builtin_amdgcn_s_waitcnt(0x4070);
         llmq_lds_barrier();
-        const bool next = g + 1 < groups;
-        if (next) {
-            stage(g + 1, nb);
+        // (no branches here: at one, the compiler moves the accumulators about; the last group's next is itself)
+        const int next = min(g + 1, groups - 1);
+        stage(next, nb);
+        ask(next);
 #pragma unroll
-            for (int r = 0; r < 4; r++) an[r] = ws[(so[r] * p.words + g + 1) * 64];
+        for (int r = 0; r < 4; r++) an[r] = ws[(so[r] * p.words + next) * 64];
+        __builtin_amdgcn_sched_barrier(0);  // the weights' loads below stay behind the copies
+        uint32_t bs[TT];
+#pragma unroll
+        for (int t = 0; t < TT; t++) bs[t] = sb[t * 64 + lane];
+        // U of the tokens' fragments at a time, the next U read while these are multiplied
+        constexpr int U = TT == 6 ? 3 : 4, H = TT / U;
+        uint4 b[2][U];
+        auto read = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < U; t++)
+                b[h & 1][t] = *reinterpret_cast<const uint4 *>(cb + (h / H * TT + h % H * U + t) * 1024 + lane * 16);
+        };
+        read(0);
+#pragma unroll
+        for (int h = 0; h < 4 * H; h++) {
+            const int j = h / H;
+            if (h + 1 < 4 * H) read(h + 1);
+            if (h % H == 0) weights(g * 4 + j + 3, a[(j + 3) % 4]);
+            // (left to itself, the compiler asks for all of these where they are used)
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < U; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    acc[r][h % H * U + t] =
+                        mma(a[j][r], b[h & 1][t], acc[r][h % H * U + t], (int)as[r], (int)bs[h % H * U + t], j);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        uint32_t bs[8];
 #pragma unroll
-        for (int t = 0; t < 8; t++) bs[t] = sb[t * 64 + lane];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int s = g * 4 + j;
-            weights(s + 2, a[(j + 2) % 3]);
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-                const uint4 b = *reinterpret_cast<const uint4 *>(cb + (j * 8 + t) * 1024 + lane * 16);
-#pragma unroll
-                for (int r = 0; r < 4; r++) acc[r][t] = mma(a[j % 3][r], b, acc[r][t], (int)as[r], (int)bs[t], j);
-            }
-        }
-        // four steps on, the ring of three has moved by one
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const uint4 x = a[1][r], y = a[2][r];
-            a[0][r] = x;
-            a[1][r] = y;
-            as[r] = an[r];
-        }
-        if (next) scales(g + 1, ns);
+        for (int r = 0; r < 4; r++) as[r] = an[r];
+        put(next, ns);
     };
-    for (int g = 0; g < groups; g += 2) {
+    int g = 0;
+    for (; g + 1 < groups; g += 2) {
         group(g, c0, c1, s0, s1);
-        if (g + 1 < groups) group(g + 1, c1, c0, s1, s0);
+        group(g + 1, c1, c0, s1, s0);
     }
+    if (g < groups) group(g, c0, c1, s0, s1);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): no copy into LDS is left behind
     const bool wide = p.n % 4 == 0 && (uintptr_t)p.out % 16 == 0 && !(p.flags & ~LLMQ_BIAS);
 #pragma unroll
-    for (int t = 0; t < 8; t++) {
+    for (int t = 0; t < TT; t++) {
         if (16 * t + c >= live) continue;
         float *row = p.out + (t0 + 16 * t + c) * p.n;
 #pragma unroll
@@ -562,28 +662,53 @@ int launch_quantize(llmq_ctx *ctx, const float *x, int64_t ldx, int64_t T, int64
     return LLMQ_OK;
 }
 
-// Tokens from which on the 256 x 128 kernel runs.
-constexpr int64_t kMany = 65;
-
 // Waves of a few-token workgroup, and groups of steps each: a wave a group as far as they go.
 int few_waves(const llmq_mat *w, int most, int *per) {
     *per = (int)((w->NG + most - 1) / most);
     return (int)((w->NG + *per - 1) / *per);
 }
 
-template <int TT, bool FUSED>
+template <int TT, int X>
 int launch_few(llmq_ctx *ctx, const Product &p, const llmq_mat *w, size_t front) {
     int per;
     const int waves = few_waves(w, few_most(TT), &per);
     const size_t sums = (size_t)waves * TT * 1024;
     const dim3 grid((unsigned)w->ntiles, (unsigned)((p.T + 16 * TT - 1) / (16 * TT)));
-    hipLaunchKernelGGL((mx4_few_kernel<TT, FUSED>), grid, dim3(64 * waves), sums > front ? sums : front, ctx->stream, p,
+    hipLaunchKernelGGL((mx4_few_kernel<TT, X>), grid, dim3(64 * waves), sums > front ? sums : front, ctx->stream, p,
                        per);
     LLMQ_HIP(hipGetLastError());
     return LLMQ_OK;
 }
 
-// The product of quantized tokens, or (codes null) of one token's floats x.
+template <int TT, int X>
+int launch_many(llmq_ctx *ctx, const Product &p) {
+    const int64_t gx = ((int64_t)p.n + kOuts - 1) / kOuts, gy = (p.T + 16 * TT - 1) / (16 * TT);
+    LLMQ_REQUIRE(gx * gy <= INT32_MAX, "mx4_linear: %lld tokens by %d outputs", (long long)p.T, p.n);
+    hipLaunchKernelGGL((mx4_many_kernel<TT, X>), dim3((unsigned)(gx * gy)), dim3(256), 0, ctx->stream, p, (int)gx,
+                       (int)gy);
+    LLMQ_HIP(hipGetLastError());
+    return LLMQ_OK;
+}
+
+// The kernel by the number of workgroups.  Few-token workgroups cost the
+// same each, however many there are, the others fill the CUs with few: up to
+// 1280 of the first are the faster (2048 outputs: 256 tokens 10.9 us against
+// 17; 11008 outputs: 128 tokens 16.4 against 14.8).  Of the two large tiles
+// the one whose workgroups, a CU's share of them after one another, are done
+// first: 2048 x 4096 x 11008 68 us with 96 tokens, 75.5 with 64; 2048 x 11008 x
+// 4096 75 and 69.
+template <int X>
+int launch_tokens(llmq_ctx *ctx, const Product &p, const llmq_mat *w) {
+    if (p.T <= 16) return launch_few<1, X>(ctx, p, w, 0);
+    if (p.T <= 32) return launch_few<2, X>(ctx, p, w, 0);
+    if (w->ntiles * ((p.T + 63) / 64) <= 1280) return launch_few<4, X>(ctx, p, w, 0);
+    const int64_t gx = (w->n + kOuts - 1) / kOuts;
+    auto cost = [&](int64_t tt) { return (gx * ((p.T + 16 * tt - 1) / (16 * tt)) + 255) / 256 * (5 * tt + 6); };
+    return cost(6) < cost(4) ? launch_many<6, X>(ctx, p) : launch_many<4, X>(ctx, p);
+}
+
+// The product of tokens given as X says: packed rows, a record, or one token's floats x.
+template <int X>
 int launch_product(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scales, const float *x, const llmq_mat *w,
                    int64_t T, float *out, const float *bias, int flags) {
     Product p;
@@ -601,17 +726,10 @@ int launch_product(llmq_ctx *ctx, const uint8_t *codes, const uint8_t *scales, c
     p.out = out;
     p.bias = bias;
     p.flags = flags;
-    if (!codes) return launch_few<1, true>(ctx, p, w, (size_t)w->NG * (16 + 256));
-    if (T >= kMany) {
-        const int64_t gx = (w->n + kOuts - 1) / kOuts, gy = (T + kTokens - 1) / kTokens;
-        LLMQ_REQUIRE(gx * gy <= INT32_MAX, "mx4_linear: %lld tokens by %lld outputs", (long long)T, (long long)w->n);
-        hipLaunchKernelGGL(mx4_many_kernel, dim3((unsigned)(gx * gy)), dim3(256), 0, ctx->stream, p, (int)gx, (int)gy);
-        LLMQ_HIP(hipGetLastError());
-        return LLMQ_OK;
-    }
-    if (T <= 16) return launch_few<1, false>(ctx, p, w, 0);
-    if (T <= 32) return launch_few<2, false>(ctx, p, w, 0);
-    return launch_few<4, false>(ctx, p, w, 0);
+    if constexpr (X == kFloats)
+        return launch_few<1, kFloats>(ctx, p, w, (size_t)w->NG * (16 + 256));
+    else
+        return launch_tokens<X>(ctx, p, w);
 }
 
 int check_epilogue(const char *name, const float *out, const float *bias, int64_t T, int flags) {
@@ -623,7 +741,11 @@ int check_epilogue(const char *name, const float *out, const float *bias, int64_
 
 }  // namespace
 
-int64_t mx4_record_bytes(int64_t T, int64_t K) { return ((T * K / 2 + 255) & ~(int64_t)255) + T * K / 32; }
+// A record of T tokens of K inputs: whole tiles of 16 and groups of 512.
+int64_t mx4_record_bytes(int64_t T, int64_t K) {
+    const int64_t values = ((T + 15) / 16 * 16) * ((K + 511) / 512 * 512);
+    return values / 2 + values / 32;
+}
 
 int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t T, float *out, const float *bias,
                       int flags, void *rec, int64_t rec_cap) {
@@ -632,7 +754,8 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
     // one token's row fits LDS beside the sums
-    if (T == 1 && w->NG * (16 + 256) <= 65536) return launch_product(ctx, nullptr, nullptr, x, w, 1, out, bias, flags);
+    if (T == 1 && w->NG * (16 + 256) <= 65536)
+        return launch_product<kFloats>(ctx, nullptr, nullptr, x, w, 1, out, bias, flags);
     const int64_t need = mx4_record_bytes(T, w->k);
     if (rec_cap < 0) {
         // the workspace is one for the context: two graphs that held it could not run side by side
@@ -644,9 +767,17 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
                      "linear_noalloc: %lld tokens x %lld inputs need %lld bytes of scratch, the maximum is %lld",
                      (long long)T, (long long)w->k, (long long)need, (long long)rec_cap);
     }
-    uint8_t *codes = static_cast<uint8_t *>(rec), *scales = codes + ((T * w->k / 2 + 255) & ~(int64_t)255);
-    RC(launch_quantize(ctx, x, w->k, T, w->k, codes, scales));
-    return launch_product(ctx, codes, scales, nullptr, w, T, out, bias, flags);
+    const int64_t tiles = (T + 15) / 16;
+    uint8_t *codes = static_cast<uint8_t *>(rec), *scales = codes + tiles * w->NG * 4096;
+    for (int64_t done = 0; done < tiles; done += 65535) {
+        const int64_t some = tiles - done < 65535 ? tiles - done : 65535;
+        hipLaunchKernelGGL(mx4_record_kernel, dim3((unsigned)w->NG, (unsigned)some), dim3(256), 0, ctx->stream,
+                           x + done * 16 * w->k, T - done * 16, (int)(w->k / 32), (int)w->NG,
+                           reinterpret_cast<uint32_t *>(codes + done * w->NG * 4096),
+                           reinterpret_cast<uint32_t *>(scales + done * w->NG * 256));
+        LLMQ_HIP(hipGetLastError());
+    }
+    return launch_product<kRecord>(ctx, codes, scales, nullptr, w, T, out, bias, flags);
 }
 
 int mx4_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *dst) {
@@ -798,7 +929,7 @@ int llmq_mx4_linear(llmq_ctx *ctx, float *out, const uint8_t *codes, const uint8
     RC(check_epilogue("mx4_linear", out, bias, T, flags));
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
-    return launch_product(ctx, codes, scales, nullptr, w, T, out, bias, flags);
+    return launch_product<kRows>(ctx, codes, scales, nullptr, w, T, out, bias, flags);
 }
 
 }  // extern "C"

@@ -189,6 +189,52 @@ def test_linear(gpu, n, k):
         m.free()
 
 
+@pytest.mark.parametrize("T,k,n", [(33, 512, 21000), (65, 2080, 11008), (300, 160, 4113), (321, 32, 4200),
+                                   (1000, 544, 1300), (4001, 1056, 350), (2048, 160, 2816), (1537, 672, 3001),
+                                   (1600, 1024, 2820)])
+def test_linear_many_workgroups(gpu, T, k, n):
+    """Sizes that the large tiles take (of 64 and of 96 tokens), odd ones
+    among them, with each epilogue, through linear, linear_noalloc and
+    mx4_linear; a NaN token and a NaN output row stay by themselves."""
+    torch, lm, ctx = gpu
+    print("mx4 many", T, k, n, flush=True)
+    rng = np.random.default_rng(T + k + n)
+    x, w = inputs(rng, T, k, n)
+    m = lm.HipMX4Matrix.from_f32(ctx, w, reduce_rows=False)
+    xv, wv = values(*quant(x)), values(*quant(w))
+    xd = dev(torch, x)
+    size = bar(xv, wv)
+    y = xv @ wv.T
+    outs = [torch.full((T + 1, n), 7.0, device="cuda") for _ in range(3)]
+    lm.linear(ctx, outs[0][:T], xd, m)
+    assert lm.lib().llmq_linear_noalloc(ctx.h, outs[1].data_ptr(), xd.data_ptr(), m.h, None, T, k, n, 0) == 0
+    codes = torch.zeros(T, k // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(T, k // 32, dtype=torch.uint8, device="cuda")
+    lm.mx4_quantize(ctx, xd, codes, scales)
+    lm.mx4_linear(ctx, outs[2][:T], codes, scales, m)
+    for o in outs:
+        assert bool((o[T] == 7.0).all()), "wrote past the last token"
+        assert np.all(np.abs(o[:T].cpu().numpy() - y) <= size)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    b, r = rng.normal(0, 1, n).astype(F), rng.normal(0, 1, (T, n)).astype(F)
+    out = torch.zeros(T, n, device="cuda")
+    lm.linear(ctx, out, xd, m, dev(torch, b))
+    assert np.all(np.abs(out.cpu().numpy() - (y + b)) <= size + 8 * 2.0 ** -24 * np.abs(b) + 2.0 ** -24 * np.abs(y + b))
+    out = dev(torch, r)
+    lm.linear(ctx, out, xd, m, resid=True)
+    assert np.all(np.abs(out.cpu().numpy() - (y + r)) <= size + 2.0 ** -23 * (np.abs(y) + np.abs(r)))
+    x[T - 2, 3], w[n - 1, 5] = np.nan, np.inf
+    m2 = lm.HipMX4Matrix.from_f32(ctx, w, reduce_rows=False)
+    lm.linear(ctx, out, dev(torch, x), m2)
+    bad = np.zeros((T, n), bool)
+    bad[T - 2], bad[:, n - 1] = True, True
+    got = out.cpu().numpy()
+    assert np.array_equal(np.isnan(got), bad)
+    assert np.array_equal(got[~bad], outs[0][:T].cpu().numpy()[~bad])
+    m.free()
+    m2.free()
+
+
 @pytest.mark.parametrize("T", [1, 3, 16, 40, 150, 300])
 @pytest.mark.parametrize("flags", ["bias", "gelu", "resid", "bias gelu", "bias resid", "bias gelu resid"])
 def test_epilogues(gpu, T, flags):
