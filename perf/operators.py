@@ -176,11 +176,12 @@ def logit_inputs(case, g):
 
 
 def library():
-    """The package and the one context that a program has: every state's calls go to one stream."""
+    """The package, and the one context and stream that a program has: every state's calls go there."""
     if not opened:
         import llm_mojo_amd as lm
 
-        opened.append((lm, lm.Context(0, torch.cuda.current_stream())))
+        stream = torch.cuda.Stream()
+        opened.append((lm, lm.Context(0, stream), stream))
     return opened[0]
 
 
@@ -188,7 +189,7 @@ def prepare(case, seed):
     g = generator(seed)
     s = {"case": case}
     if own:
-        s["lm"], s["ctx"] = library()
+        s["lm"], s["ctx"], s["stream"] = library()
     if case["kind"] in ("step", "store"):
         kv, hd, page = case["kv"], case["hd"], case["page"]
         s["length"], s["table"], n_pages = paged(case, seed, g)
@@ -214,7 +215,9 @@ def prepare(case, seed):
             s["all"] = torch.arange(n, dtype=torch.int32, device="cuda")
             s["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads) if case["bias"] else None
             if own:
+                s["stream"].wait_stream(torch.cuda.current_stream())
                 s["cache"].store(0, k, v, seq, pos, s["table"])
+                torch.cuda.current_stream().wait_stream(s["stream"])
                 s["work"] = torch.empty(s["cache"].work_bytes(n, heads), dtype=torch.uint8, device="cuda")
                 s["ko"], s["vo"] = torch.empty(n, kv, hd, device="cuda"), torch.empty(n, kv, hd, device="cuda")
             else:
@@ -236,7 +239,9 @@ def prepare(case, seed):
         s["resid"] = normal(g, t, n) if case["resid"] else None
         s["out"] = torch.zeros(t, n, device="cuda")
         if own:
+            s["stream"].wait_stream(torch.cuda.current_stream())
             s["w"] = s["lm"].HipMX4Matrix.from_f32(s["ctx"], w, reduce_rows=False)
+            torch.cuda.current_stream().wait_stream(s["stream"])
         else:
             s["w"] = pack(*mx4(w))
     else:
@@ -402,7 +407,8 @@ def run(s):
     if c["kind"] == "linear":
         if own:
             if c["resid"]:
-                s["out"].copy_(s["resid"])
+                with torch.cuda.stream(s["stream"]):
+                    s["out"].copy_(s["resid"])
             s["lm"].linear(s["ctx"], s["out"], s["x"], s["w"], s["b"], resid=c["resid"], gelu=c["gelu"])
             return s["out"]
         return plain_linear(s)
