@@ -332,9 +332,9 @@ LLMQ_API int llmq_ikv_export(llmq_ctx *ctx, const llmq_kv *kv, int8_t *k, int8_t
  * graph follows them.
  *
  * Held per position and cached head: LLMQ_PKV_INT8 int8 codes with a float32
- * scale for the key and for the value, as QuantKV[8] (kvcache.mojo:248-385;
- * a row with a NaN or an infinity reads back as NaN, one below 2^-120 as
- * zeros); LLMQ_PKV_F16 float16 values (nearest even, finite values past
+ * scale for the key and for the value, as QuantKV[8] (kvcache.mojo:248-385)
+ * but for a scale's last bit: max|x| times the float 1 / 127 (a row with a
+ * NaN or an infinity reads back as NaN, one below 2^-120 as zeros); LLMQ_PKV_F16 float16 values (nearest even, finite values past
  * 65504 saturate).  page: 64 to 4096 positions, a multiple of 64; head_dim
  * 64 or 128 (LLMQ_EUNSUPPORTED otherwise). */
 typedef struct llmq_pkv llmq_pkv;

@@ -44,14 +44,15 @@ __device__ __forceinline__ int64_t head_row(const Layer &c, int page, int head) 
     return ((int64_t)page * c.n_kv + head) * c.page;
 }
 
-// QuantKV.store's quantisation of a row (kvcache.mojo:333-342): s = max|x| /
-// 127 (1 for a row of zeros), codes round(x / s) away from zero at ties, kept
+// QuantKV.store's quantisation of a row (kvcache.mojo:333-342), but for the
+// last bit of a scale: s = max|x| / 127 as a product with the rounded 1 / 127
+// (1 for a row of zeros), codes round(x (1 / s)) away from zero at ties, kept
 // plus kBias.  A row with a NaN or an infinity (largest: infinity) gets the
 // scale NaN; one below 2^-120, whose reciprocal scale is infinite, is a row of
 // zeros.
 __device__ __forceinline__ float row_scale(float largest) {
     if (largest == INFINITY) return __uint_as_float(0x7fc00000u);
-    return largest < 0x1p-120f ? 1.0f : largest / 127.0f;
+    return largest < 0x1p-120f ? 1.0f : largest * (1.0f / 127.0f);
 }
 __device__ __forceinline__ int row_code(float x, float inv) { return llmq_to_int(roundf(x * inv)) + kBias; }
 

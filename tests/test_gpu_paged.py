@@ -1,8 +1,9 @@
 """The paged key / value cache and one token's attention over it (llmq_pkv_*)
 against its definition in float64.
 
-Rows: what fetch gives is compared bit by bit with QuantKV.store's rounding
-(or float16's).  Attention: over the fetched rows in float64.  With S the sum
+Rows: what fetch gives is compared bit by bit with the definition's rounding
+(scale max|x| times the float 1 / 127, codes away from zero at ties; or
+float16's).  Attention: over the fetched rows in float64.  With S the sum
 of |q_d k_d| times |scale| (a bar has no sign), a score is off by at most
   d = S (2^-22 + (hd + 8) 2^-24) + 4 2^-24 |s| (+ 2^-22 cap; + 2^-23 |bias|)
 (queries held to 22 bits, the products added in float32, a few roundings of
@@ -28,7 +29,7 @@ def held(kind, x):
     if kind == "f16":
         return np.clip(x, -65504, 65504).astype(np.float16).astype(np.float32)
     m = np.abs(x).max(-1, keepdims=True)
-    s = np.where(m < np.float32(2.0 ** -120), np.float32(1), m / np.float32(127)).astype(np.float32)
+    s = np.where(m < np.float32(2.0 ** -120), np.float32(1), m * (np.float32(1) / np.float32(127))).astype(np.float32)
     y = x * (np.float32(1) / s)
     return (np.sign(y) * np.floor(np.abs(y) + np.float32(0.5))).astype(np.float32) * s
 
