@@ -789,7 +789,10 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         for (int i = 0; i < NT * 4; i++) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sv[i], kLog2e, -ref2));
             l += p;
-            const float y = ELEM == 1 ? p * (vs[i >> 2][i & 3] * unit) : p * unit;
+            float y = ELEM == 1 ? p * (vs[i >> 2][i & 3] * unit) : p * unit;
+            // rounded to 32 bits once, for both rows: the product straight to 16 bits would now and then be another
+            // float16 than the one below, and the rows no longer add up
+            asm volatile("" : "+v"(y));
             const float hi = (float)(_Float16)y;
             // row n: y rounded; row n ^ 8: what that leaves times 2^11 (exact)
             wf[i] = (_Float16)fmaf(hi, wr, y * wg);

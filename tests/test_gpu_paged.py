@@ -261,6 +261,29 @@ def test_attend_long_and_ragged(gpu, kind):
     check(c, 4)
 
 
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("kind", KINDS)
+def test_attend_weights_hold_22_bits(gpu, kind, n):
+    """Sequences of one or two positions, 32000 weights: with so few terms a
+    weight's own error shows.  A weight is held to 22 bits (2^-22 of it), its
+    scale, exponential, sum and quotient round a few times: 2^-20 of sum p |v|
+    in all, besides the scores' error, which one position does not have."""
+    torch, lm, ctx = gpu
+    rows, heads = 4000, 8
+    c = Case(gpu, kind, 64, heads, [n] * rows)
+    q, got = c.attend(heads)
+    order = np.lexsort((c.pos, c.seq))
+    k, v = (held(kind, x)[order].reshape(rows, n, heads, 64).astype(np.float64) for x in (c.k, c.v))
+    s = np.einsum("rnhd,rhd->rnh", k, q.astype(np.float64)) / 8
+    d = np.einsum("rnhd,rhd->rnh", np.abs(k), np.abs(q.astype(np.float64))) / 8 * (2.0 ** -22 + 72 * 2.0 ** -24)
+    p = np.exp(s - s.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    out = np.einsum("rnh,rnhd->rhd", p, v)
+    size = np.einsum("rnh,rnhd->rhd", p, np.abs(v))
+    bar = (2.0 ** -20 + (2 * d.max(1) if n > 1 else 0 * d.max(1)))[..., None] * size + 1e-37
+    assert np.max(np.abs(got - out) / bar) <= 1.0
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_attend_many_rows(gpu, kind):
     rng = np.random.default_rng(5)
