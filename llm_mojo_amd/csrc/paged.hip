@@ -336,6 +336,9 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.402823466e38f;
+// Cache policy of loads whose lines are read once (nt): 342 MB of float16 64.4 us with it, 70.5 without; 1118 MB of
+// int8 221 and 226.
+constexpr int kOnce = 2;
 
 // Eight int8 codes as float16, exactly: byte u = code + 128 under the
 // exponent byte 0x64 is 1024 + u, less 1152.
@@ -558,7 +561,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
 #pragma unroll
             for (int i = 0; i < NC; i++) {
                 const auto y = __builtin_amdgcn_raw_buffer_load_b128(rk, n * HD * ELEM + q * 16,
-                                                                     t * 16 * HD * ELEM + i * 64, 0);
+                                                                     t * 16 * HD * ELEM + i * 64, kOnce);
 #pragma unroll
                 for (int e = 0; e < 4; e++) kr[t * NC + i][e] = y[e];
             }
@@ -575,11 +578,11 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         for (int d = 0; d < ND; d++) {
             const int vo = (n * B + q * 8) * ELEM, so = d * 16 * B * ELEM;
             if constexpr (ELEM == 1) {
-                const auto y = __builtin_amdgcn_raw_buffer_load_b64(rv, vo, so, 0);
+                const auto y = __builtin_amdgcn_raw_buffer_load_b64(rv, vo, so, kOnce);
                 vr[d][0] = y[0];
                 vr[d][1] = y[1];
             } else {
-                const auto y = __builtin_amdgcn_raw_buffer_load_b128(rv, vo, so, 0);
+                const auto y = __builtin_amdgcn_raw_buffer_load_b128(rv, vo, so, kOnce);
 #pragma unroll
                 for (int e = 0; e < 4; e++) vr[d][e] = y[e];
             }
