@@ -37,7 +37,7 @@ struct Span {
 };
 __device__ __forceinline__ Span span_of(const int64_t *off, int64_t len, int64_t r) {
     const int64_t lo = off[r], hi = off[r + 1];
-    return Span{lo < 0 ? 0 : lo, hi > len ? len : hi};
+    return Span{lo < 0 ? 0 : (lo > len ? len : lo), hi > len ? len : hi};  // (positions past lo do not wrap)
 }
 
 struct Best {

@@ -175,6 +175,20 @@ def test_offsets_outside_the_lists(gpu):
     assert same(got, o)
 
 
+@pytest.mark.parametrize("lo", [2 ** 63 - 1, 2 ** 63 - 300, 41])
+def test_offsets_at_the_type_s_end(gpu, lo):
+    """A row that begins past its list, also where its next entries' positions would wrap, is empty."""
+    rng = np.random.default_rng(11)
+    x = rng.normal(0, 1, (2, 600)).astype(F)
+    hist = rng.integers(0, 600, 40).astype(np.int32)
+    one = np.full(2, 1.5, F)
+    got, _ = run(gpu, x, hist=hist, rep=one, hoff=np.array([0, lo, 2 ** 63 - 1], np.int64),
+                 bias=(hist[:10], x[0, :10], np.array([0, lo, 2 ** 63 - 1], np.int64)))
+    o, _ = want(x, hist=hist, rep=one, hoff=np.array([0, 40, 40], np.int64),
+                bias=(hist[:10], x[0, :10], np.array([0, 10, 10], np.int64)))
+    assert same(got, o)
+
+
 def test_empty_lists(gpu):
     torch, lm, ctx = gpu
     x = np.random.default_rng(6).normal(0, 1, (2, 100)).astype(F)
