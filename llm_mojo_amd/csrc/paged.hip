@@ -45,15 +45,17 @@ __device__ __forceinline__ int64_t head_row(const Layer &c, int page, int head) 
 }
 
 // QuantKV.store's quantisation of a row (kvcache.mojo:333-342), but for the
-// last bit of a scale: s = max|x| / 127 as a product with the rounded 1 / 127
-// (1 for a row of zeros), codes round(x (1 / s)) away from zero at ties, kept
-// plus kBias.  A row with a NaN or an infinity (largest: infinity) gets the
-// scale NaN; one below 2^-120, whose reciprocal scale is infinite, is a row of
-// zeros.
+// last bit of a scale: s = max|x| / 127 as a product with the rounded 1 / 127,
+// codes round(x (1 / s)) away from zero at ties, kept plus kBias.  A row with a
+// NaN or an infinity (largest: infinity) gets the scale NaN; one below 2^-120,
+// whose reciprocal scale is infinite, is a row of zeros.  Their scale is 0, not
+// QuantKV's 1: the attention's weights carry the scales relative to the
+// largest, beside which those of small values would vanish.
 __device__ __forceinline__ float row_scale(float largest) {
     if (largest == INFINITY) return __uint_as_float(0x7fc00000u);
-    return largest < 0x1p-120f ? 1.0f : largest * (1.0f / 127.0f);
+    return largest < 0x1p-120f ? 0.0f : largest * (1.0f / 127.0f);
 }
+__device__ __forceinline__ float inverse_of(float scale) { return scale > 0.0f ? 1.0f / scale : 0.0f; }
 __device__ __forceinline__ int row_code(float x, float inv) { return llmq_to_int(roundf(x * inv)) + kBias; }
 
 __device__ __forceinline__ uint16_t half_bits(float x) {
@@ -73,7 +75,7 @@ __device__ __forceinline__ float encode_row(const float (&x)[HD / 64], int (&cod
             bad += x[i] - x[i];  // NaN for NaN and infinities
         }
         m = llmq_wave_max_all(bad != 0.0f || bad != bad ? INFINITY : m);
-        const float s = row_scale(m), inv = 1.0f / s;
+        const float s = row_scale(m), inv = inverse_of(s);
 #pragma unroll
         for (int i = 0; i < HD / 64; i++) code[i] = row_code(x[i], inv);
         return s;
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(kRows *kLanes) void pkv_store_kernel(Layer c, const
                             bad += x[s][i][e] - x[s][i][e];  // NaN for NaN and infinities
                         }
                     m = eighth_max(bad != 0.0f || bad != bad ? INFINITY : m);
-                    const float scale = row_scale(m), inv = 1.0f / scale;
+                    const float scale = row_scale(m), inv = inverse_of(scale);
 #pragma unroll
                     for (int i = 0; i < NP; i++) {
                         uint32_t u = 0;

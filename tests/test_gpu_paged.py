@@ -321,6 +321,18 @@ def test_attend_uneven_value_scales(gpu):
     check(c, 2)
 
 
+def test_attend_zero_rows_among_small(gpu):
+    """Rows of zeros, whose int8 scale says nothing, beside values near 2^-60."""
+    torch, lm, ctx = gpu
+    c = Case(gpu, "int8", 64, 1, [100])
+    at = c.rows(0)
+    c.v[at] *= np.float32(2.0 ** -60)
+    c.v[at[::3]] = 0
+    c.k[at[1::3]] = 0
+    c.cache.store(0, dev(torch, c.k), dev(torch, c.v), dev(torch, c.seq), dev(torch, c.pos), c.table)
+    check(c, 2)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_attend_lengths_past_the_table_and_bad_pages(gpu, kind):
     torch, lm, ctx = gpu
