@@ -205,7 +205,7 @@ class Context:
     def __init__(self, device=0, stream=None):
         h = ctypes.c_void_p()
         check(lib().llmq_init(device, ctypes.byref(h)))
-        self.h = h
+        self.h, self.device = h, device
         if stream is not None:
             self.set_stream(stream)
 

@@ -270,6 +270,7 @@ int llmq_adjust_logits(llmq_ctx *ctx, float *out, int64_t ldo, const float *logi
     LLMQ_REQUIRE(!pick || rows == 0 || (work && work_bytes >= want), "adjust_logits: %lld bytes of work, %lld needed",
                  (long long)work_bytes, (long long)want);
     if (rows == 0) return LLMQ_OK;
+    LLMQ_REQUIRE(!pick || (uintptr_t)work % 16 == 0, "adjust_logits: work is 16-byte aligned");
     DeviceGuard guard(ctx);
     const int chunk = chunk_of(rows, V), n = (int)((V + chunk - 1) / chunk);
     Best *parts = pick ? static_cast<Best *>(work) : nullptr;

@@ -782,20 +782,25 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
 
 int mx4_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *dst) {
     DeviceGuard guard(ctx);
-    const int64_t nb = m->k / 32, tile = row >> 4, r = row & 15;
-    std::vector<uint8_t> c((size_t)m->NG * 4096), s((size_t)m->NG * 256);
-    LLMQ_HIP(hipMemcpyAsync(c.data(), m->codes + tile * m->NG * 4096, c.size(), hipMemcpyDeviceToHost, ctx->stream));
-    LLMQ_HIP(hipMemcpyAsync(s.data(), reinterpret_cast<const uint8_t *>(m->scales) + tile * m->NG * 256, s.size(),
-                            hipMemcpyDeviceToHost, ctx->stream));
-    LLMQ_HIP(hipStreamSynchronize(ctx->stream));
-    static const float val[16] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f,
-                                  -0.0f, -0.5f, -1.0f, -1.5f, -2.0f, -3.0f, -4.0f, -6.0f};
-    for (int64_t b = 0; b < nb; b++) {
-        const Place at = place_of(m, r, b);  // the row within its own tile
-        const int e = s[(size_t)at.scale];
-        const float sc = e == 255 ? NAN : ldexpf(1.0f, e - 127);
-        for (int j = 0; j < 32; j++)
-            dst[b * 32 + j] = val[(c[(size_t)at.code * 16 + j / 2] >> (4 * (j & 1))) & 15] * sc;
+    try {
+        const int64_t nb = m->k / 32, tile = row >> 4, r = row & 15;
+        std::vector<uint8_t> c((size_t)m->NG * 4096), s((size_t)m->NG * 256);
+        LLMQ_HIP(hipMemcpyAsync(c.data(), m->codes + tile * m->NG * 4096, c.size(), hipMemcpyDeviceToHost,
+                                ctx->stream));
+        LLMQ_HIP(hipMemcpyAsync(s.data(), reinterpret_cast<const uint8_t *>(m->scales) + tile * m->NG * 256, s.size(),
+                                hipMemcpyDeviceToHost, ctx->stream));
+        LLMQ_HIP(hipStreamSynchronize(ctx->stream));
+        static const float val[16] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f,
+                                      -0.0f, -0.5f, -1.0f, -1.5f, -2.0f, -3.0f, -4.0f, -6.0f};
+        for (int64_t b = 0; b < nb; b++) {
+            const Place at = place_of(m, r, b);  // the row within its own tile
+            const int e = s[(size_t)at.scale];
+            const float sc = e == 255 ? NAN : ldexpf(1.0f, e - 127);
+            for (int j = 0; j < 32; j++)
+                dst[b * 32 + j] = val[(c[(size_t)at.code * 16 + j / 2] >> (4 * (j & 1))) & 15] * sc;
+        }
+    } catch (const std::bad_alloc &) {
+        return llmq_set_error(LLMQ_ENOMEM, "dequant_row: out of host memory");
     }
     return LLMQ_OK;
 }

@@ -1024,6 +1024,7 @@ int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int p
                  "pkv_create: pages of %d positions (64 to 4096, a multiple of 64)", page);
     if (head_dim != 64 && head_dim != 128)
         return llmq_set_error(LLMQ_EUNSUPPORTED, "pkv_create: head_dim %d (64 or 128)", head_dim);
+    LLMQ_REQUIRE(!ctx_capturing(ctx), "pkv_create: not under graph capture");
     const double total = (double)n_layer * (double)n_pages * n_kv * page * head_dim * 2.0;
     LLMQ_REQUIRE(total < 1e15, "pkv_create: %g elements", total);
     llmq_pkv *kv = new (std::nothrow) llmq_pkv();
@@ -1048,7 +1049,8 @@ int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int p
     if (hipMemsetAsync(kv->k, zero, n, ctx->stream) != hipSuccess ||
         hipMemsetAsync(kv->v, zero, n, ctx->stream) != hipSuccess ||
         (scales && (hipMemsetAsync(kv->ks, 0, ns, ctx->stream) != hipSuccess ||
-                    hipMemsetAsync(kv->vs, 0, ns, ctx->stream) != hipSuccess))) {
+                    hipMemsetAsync(kv->vs, 0, ns, ctx->stream) != hipSuccess)) ||
+        hipStreamSynchronize(ctx->stream) != hipSuccess) {  // other streams may use it at once
         llmq_pkv_free(kv);
         return llmq_set_error(LLMQ_EHIP, "pkv_create: clearing the cache failed");
     }

@@ -194,8 +194,8 @@ class HipMX4Matrix:
             src = np.ascontiguousarray(src, np.float32)
             check(lib().llmq_mat_from_f32_mx4(ctx.h, hptr(src), rows, cols, 1 if reduce_rows else 0, ctypes.byref(h)))
         else:
-            if str(src.dtype) != "torch.float32" or not src.is_cuda or not src.is_contiguous():
-                raise ValueError("from_f32: a contiguous float32 tensor on the GPU")
+            if str(src.dtype) != "torch.float32" or src.get_device() != ctx.device or not src.is_contiguous():
+                raise ValueError(f"from_f32: a contiguous float32 tensor on GPU {ctx.device}")
             check(lib().llmq_mat_from_f32_mx4_device(ctx.h, dptr(src), rows, cols, 1 if reduce_rows else 0,
                                                      ctypes.byref(h)))
         return cls(ctx, h)
@@ -244,38 +244,43 @@ class HipMX4Matrix:
             pass
 
 
-def _mx4_rows(x, codes, scales):
+def _mx4_rows(ctx, x, codes, scales):
     """(rows, columns, row stride) of x[T, K] with packed codes[T, K / 2] and scales[T, K / 32]."""
     T, K = x.shape
-    if str(x.dtype) != "torch.float32" or not x.is_cuda or (x.numel() and x.stride(1) != 1):
-        raise ValueError("mx4: float32 rows in one piece on the GPU")
-    _mx4_packed(codes, scales, T, K)
+    if str(x.dtype) != "torch.float32" or x.get_device() != ctx.device or (x.numel() and x.stride(1) != 1):
+        raise ValueError(f"mx4: float32 rows in one piece on GPU {ctx.device}")
+    _mx4_packed(ctx, codes, scales, T, K)
     return T, K, x.stride(0) if T > 1 else max(x.stride(0), K)
 
 
-def _mx4_packed(codes, scales, T, K):
+def _mx4_packed(ctx, codes, scales, T, K):
     for t, shape in ((codes, (T, K // 2)), (scales, (T, K // 32))):
-        if str(t.dtype) != "torch.uint8" or not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != shape:
-            raise ValueError(f"mx4: contiguous uint8 codes [{T}, {K // 2}] and scales [{T}, {K // 32}] on the GPU")
+        if (str(t.dtype) != "torch.uint8" or t.get_device() != ctx.device or not t.is_contiguous()
+                or tuple(t.shape) != shape):
+            raise ValueError(f"mx4: contiguous uint8 codes [{T}, {K // 2}] and scales [{T}, {K // 32}] on GPU "
+                             f"{ctx.device}")
 
 
 def mx4_quantize(ctx, x, codes, scales):
     """Rows x[T, K] to packed e2m1 codes[T, K / 2] and e8m0 scales[T, K / 32] (uint8 tensors)."""
-    T, K, ld = _mx4_rows(x, codes, scales)
+    T, K, ld = _mx4_rows(ctx, x, codes, scales)
     check(lib().llmq_mx4_quantize(ctx.h, dptr(x), ld, T, K, dptr(codes), dptr(scales)))
 
 
 def mx4_dequantize(ctx, codes, scales, out):
     """The values that packed rows stand for, into out[T, K]."""
-    T, K, ld = _mx4_rows(out, codes, scales)
+    T, K, ld = _mx4_rows(ctx, out, codes, scales)
     check(lib().llmq_mx4_dequantize(ctx.h, dptr(codes), dptr(scales), T, K, dptr(out), ld))
 
 
 def mx4_linear(ctx, out, codes, scales, w, bias=None, resid=False, gelu=False):
     """linear over rows that mx4_quantize left: out (+)= act(x @ w^T + bias)."""
-    _mx4_packed(codes, scales, codes.shape[0], w.cols)
-    if str(out.dtype) != "torch.float32" or not out.is_contiguous() or tuple(out.shape) != (codes.shape[0], w.rows):
-        raise ValueError(f"mx4_linear: a contiguous float32 out[{codes.shape[0]}, {w.rows}]")
+    _mx4_packed(ctx, codes, scales, codes.shape[0], w.cols)
+    for t, shape in ((out, (codes.shape[0], w.rows)), (bias, (w.rows,))):
+        if t is not None and (str(t.dtype) != "torch.float32" or not t.is_contiguous() or tuple(t.shape) != shape
+                              or t.get_device() != ctx.device):
+            raise ValueError(f"mx4_linear: a contiguous float32 out[{codes.shape[0]}, {w.rows}] and bias[{w.rows}] on "
+                             f"GPU {ctx.device}")
     flags = (LLMQ_BIAS if bias is not None else 0) | (LLMQ_GELU if gelu else 0) | (LLMQ_RESID if resid else 0)
     check(lib().llmq_mx4_linear(ctx.h, dptr(out), dptr(codes), dptr(scales), w.h, dptr(bias), codes.shape[0], w.cols,
                                 w.rows, flags))

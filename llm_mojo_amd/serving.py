@@ -36,23 +36,23 @@ def _torch():
     return torch
 
 
-def _rows(t, heads, hd, name):
-    """Row stride of float32 [rows, heads, hd] (or [rows, heads * hd]) with whole rows in one piece."""
+def _rows(t, heads, hd, dev, name):
+    """Row stride of float32 [rows, heads, hd] (or [rows, heads * hd]) on GPU dev with whole rows in one piece."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 3:
         ok = shape[1] == heads and shape[2] == hd and stride[2] == 1 and (heads == 1 or stride[1] == hd)
     else:
         ok = len(shape) == 2 and shape[1] == heads * hd and stride[1] == 1
-    if not ok or t.dtype is not torch.float32 or not t.is_cuda:
-        raise ValueError(f"{name}: a float32 tensor on the GPU of rows of {heads} heads of {hd} in one piece, "
+    if not ok or t.dtype is not torch.float32 or t.get_device() != dev:
+        raise ValueError(f"{name}: a float32 tensor on GPU {dev} of rows of {heads} heads of {hd} in one piece, "
                          f"got {tuple(shape)} with strides {stride}")
     return stride[0] if shape[0] > 1 else max(stride[0], heads * hd)
 
 
-def _ints(t, shape, name):
+def _ints(t, shape, dev, name):
     """Address of a contiguous int32 tensor of that shape."""
-    if t.shape != shape or t.dtype is not torch.int32 or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name}: a contiguous int32 tensor of shape {shape} on the GPU")
+    if t.shape != shape or t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: a contiguous int32 tensor of shape {shape} on GPU {dev}")
     return t.data_ptr()
 
 
@@ -74,6 +74,7 @@ class PagedKV:
         check(lib().llmq_pkv_create(ctx.h, PKV_TYPES[kind], n_layer, n_pages, page, n_kv, head_dim, ctypes.byref(h)))
         self.h = h
         self._scale = 1.0 / math.sqrt(head_dim)
+        self._dev = ctx.device
 
     def nbytes(self):
         return lib().llmq_pkv_nbytes(self.h)
@@ -83,13 +84,13 @@ class PagedKV:
         return lib().llmq_pkv_work_bytes(self.h, rows, n_head)
 
     def _move(self, call, layer, k, v, seq, pos, table):
-        ld = _rows(k, self.n_kv, self.head_dim, "k")
+        ld = _rows(k, self.n_kv, self.head_dim, self._dev, "k")
         n = k.shape[0]
-        if v.shape[0] != n or _rows(v, self.n_kv, self.head_dim, "v") != ld:
+        if v.shape[0] != n or _rows(v, self.n_kv, self.head_dim, self._dev, "v") != ld:
             raise ValueError("k and v: rows of one number and stride")
         n_seq, width = table.shape
-        check(call(self.ctx.h, self.h, layer, k.data_ptr(), v.data_ptr(), ld, n, _ints(seq, (n,), "seq"),
-                   _ints(pos, (n,), "pos"), _ints(table, (n_seq, width), "table"), n_seq, width))
+        check(call(self.ctx.h, self.h, layer, k.data_ptr(), v.data_ptr(), ld, n, _ints(seq, (n,), self._dev, "seq"),
+                   _ints(pos, (n,), self._dev, "pos"), _ints(table, (n_seq, width), self._dev, "table"), n_seq, width))
 
     def store(self, layer, k, v, seq, pos, table):
         """Rows of keys and values ([T, n_kv, head_dim]) at positions pos[t] of
@@ -104,16 +105,16 @@ class PagedKV:
         """(query heads, out's and q's row strides, the slopes' address, work's address and bytes)."""
         hd = self.head_dim
         n_head = q.shape[1] if q.dim() == 3 else q.shape[1] // hd
-        ldq, ldo = _rows(q, n_head, hd, "q"), _rows(out, n_head, hd, "out")
+        ldq, ldo = _rows(q, n_head, hd, self._dev, "q"), _rows(out, n_head, hd, self._dev, "out")
         if out.shape[0] != q.shape[0]:
             raise ValueError("out and q: rows of one number")
-        if not work.is_cuda or not work.is_contiguous():
-            raise ValueError("work: contiguous memory on the GPU")
+        if work.get_device() != self._dev or not work.is_contiguous():
+            raise ValueError(f"work: contiguous memory on GPU {self._dev}")
         sl = None
         if slopes is not None:
             if (slopes.dtype is not torch.float32 or slopes.shape != (n_head,) or not slopes.is_contiguous()
-                    or not slopes.is_cuda):
-                raise ValueError(f"slopes: {n_head} contiguous float32 values on the GPU")
+                    or slopes.get_device() != self._dev):
+                raise ValueError(f"slopes: {n_head} contiguous float32 values on GPU {self._dev}")
             sl = slopes.data_ptr()
         return n_head, ldo, ldq, sl, work.data_ptr(), work.nbytes
 
@@ -125,7 +126,8 @@ class PagedKV:
         n, width = q.shape[0], table.shape[1]
         n_head, ldo, ldq, sl, w, nw = self._queries(out, q, slopes, work)
         check(lib().llmq_pkv_attend(self.ctx.h, self.h, layer, out.data_ptr(), ldo, q.data_ptr(), ldq, n, n_head,
-                                    _ints(length, (n,), "length"), _ints(table, (n, width), "table"), width,
+                                    _ints(length, (n,), self._dev, "length"),
+                                    _ints(table, (n, width), self._dev, "table"), width,
                                     self._scale if scale is None else scale, cap, sl, w, nw))
 
     def step(self, layer, out, q, k, v, pos, table, work, scale=None, cap=0.0, slopes=None):
@@ -135,12 +137,13 @@ class PagedKV:
         qkv tensor)."""
         n, width = q.shape[0], table.shape[1]
         n_head, ldo, ldq, sl, w, nw = self._queries(out, q, slopes, work)
-        ldk, ldv = _rows(k, self.n_kv, self.head_dim, "k"), _rows(v, self.n_kv, self.head_dim, "v")
+        ldk = _rows(k, self.n_kv, self.head_dim, self._dev, "k")
+        ldv = _rows(v, self.n_kv, self.head_dim, self._dev, "v")
         if k.shape[0] != n or v.shape[0] != n or (n > 1 and not ldk == ldv == ldq):
             raise ValueError("q, k and v: rows of one number and stride")
         check(lib().llmq_pkv_step(self.ctx.h, self.h, layer, out.data_ptr(), ldo, q.data_ptr(), k.data_ptr(),
-                                  v.data_ptr(), ldq, n, n_head, _ints(pos, (n,), "pos"),
-                                  _ints(table, (n, width), "table"), width,
+                                  v.data_ptr(), ldq, n, n_head, _ints(pos, (n,), self._dev, "pos"),
+                                  _ints(table, (n, width), self._dev, "table"), width,
                                   self._scale if scale is None else scale, cap, sl, w, nw))
 
     def free(self):
@@ -160,10 +163,10 @@ def logits_work_bytes(rows, V):
     return lib().llmq_adjust_logits_work_bytes(rows, V)
 
 
-def _vec(t, dtype, n, name):
+def _vec(t, dtype, n, dev, name):
     """Address of a contiguous 1-d tensor of n elements."""
-    if t.shape != (n,) or t.dtype is not dtype or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name}: a contiguous {dtype} tensor of {n} on the GPU")
+    if t.shape != (n,) or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of {n} on GPU {dev}")
     return t.data_ptr()
 
 
@@ -177,38 +180,41 @@ def adjust_logits(ctx, out, logits, history=None, repetition=None, presence=None
     t = torch or _torch()
     f32, i32, i64 = t.float32, t.int32, t.int64
     rows, V = logits.shape
+    dev = ctx.device
     ld = []
     for t in (out, logits):
         stride = t.stride()
-        if t.shape != (rows, V) or t.dtype is not f32 or stride[1] != 1 or not t.is_cuda:
-            raise ValueError(f"logits and out: float32 [{rows}, {V}] on the GPU with rows in one piece")
+        if t.shape != (rows, V) or t.dtype is not f32 or stride[1] != 1 or t.get_device() != dev:
+            raise ValueError(f"logits and out: float32 [{rows}, {V}] on GPU {dev} with rows in one piece")
         ld.append(stride[0] if rows > 1 else max(stride[0], V))
     r = LogitRules()
     if history is not None:
         ids, offsets = history
         r.history_len = n = ids.shape[0]
-        r.history, r.history_offsets = _vec(ids, i32, n, "history"), _vec(offsets, i64, rows + 1, "history offsets")
+        r.history = _vec(ids, i32, n, dev, "history")
+        r.history_offsets = _vec(offsets, i64, rows + 1, dev, "history offsets")
     if repetition is not None:
-        r.repetition = _vec(repetition, f32, rows, "repetition")
+        r.repetition = _vec(repetition, f32, rows, dev, "repetition")
     if presence is not None:
-        r.presence = _vec(presence, f32, rows, "presence")
+        r.presence = _vec(presence, f32, rows, dev, "presence")
     if frequency is not None:
-        r.frequency = _vec(frequency, f32, rows, "frequency")
+        r.frequency = _vec(frequency, f32, rows, dev, "frequency")
     if bias is not None:
         ids, values, offsets = bias
         r.bias_len = n = ids.shape[0]
-        r.bias_ids, r.bias = _vec(ids, i32, n, "bias ids"), _vec(values, f32, n, "biases")
-        r.bias_offsets = _vec(offsets, i64, rows + 1, "bias offsets")
+        r.bias_ids, r.bias = _vec(ids, i32, n, dev, "bias ids"), _vec(values, f32, n, dev, "biases")
+        r.bias_offsets = _vec(offsets, i64, rows + 1, dev, "bias offsets")
     if mask is not None:
         words = mask.shape[1]
         stride = mask.stride()
-        if mask.shape[0] != rows or 32 * words < V or stride[1] != 1 or mask.dtype is not i32 or not mask.is_cuda:
-            raise ValueError(f"mask: int32 words on the GPU, {rows} rows of {V} bits")
+        if (mask.shape[0] != rows or 32 * words < V or stride[1] != 1 or mask.dtype is not i32
+                or mask.get_device() != dev):
+            raise ValueError(f"mask: int32 words on GPU {dev}, {rows} rows of {V} bits")
         r.mask, r.mask_ld = mask.data_ptr(), stride[0] if rows > 1 else max(stride[0], words)
     w, nw, at = None, 0, None
     if pick is not None:
-        if work is None or not work.is_cuda or not work.is_contiguous():
-            raise ValueError("pick: contiguous work memory on the GPU")
-        w, nw, at = work.data_ptr(), work.nbytes, _vec(pick, i64, rows, "pick")
+        if work is None or work.get_device() != dev or not work.is_contiguous():
+            raise ValueError(f"pick: contiguous work memory on GPU {dev}")
+        w, nw, at = work.data_ptr(), work.nbytes, _vec(pick, i64, rows, dev, "pick")
     check(lib().llmq_adjust_logits(ctx.h, out.data_ptr(), ld[0], logits.data_ptr(), ld[1], rows, V, ctypes.byref(r), at,
                                    w, nw))
