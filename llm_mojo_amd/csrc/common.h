@@ -585,6 +585,14 @@ constexpr uint32_t kLlmqOOB = 0x80000000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t llmq_rsrc(const void *p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
 }
+// Four floats by a streaming load (nt): for rows that a kernel reads once and
+// whose lines need not stay in the caches.
+__device__ __forceinline__ void llmq_load4_once(const float *p, float *x) {
+    typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
+    const v4u y = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(p));
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = y[i];
+}
 __device__ __forceinline__ uint4 llmq_bload16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
     const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0);
     return make_uint4(v[0], v[1], v[2], v[3]);

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
         const int v = v0 + 4 * (tid + kThreads * k);
         bits[k] = 15;
         if (v + 4 <= V) {
-            x[k] = *reinterpret_cast<const Float4 *>(src + v);
+            llmq_load4_once(src + v, x[k].x);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) x[k].x[i] = v + i < V ? src[v + i] : 0.0f;

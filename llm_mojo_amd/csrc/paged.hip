@@ -206,7 +206,7 @@ __global__ __launch_bounds__(kRows *kLanes) void pkv_store_kernel(Layer c, const
             for (int s = 0; s < 2; s++)
 #pragma unroll
                 for (int i = 0; i < NP; i++)
-                    *reinterpret_cast<Floats4 *>(x[s][i]) = *reinterpret_cast<const Floats4 *>(src[s] + 32 * i + 4 * j);
+                    llmq_load4_once(src[s] + 32 * i + 4 * j, x[s][i]);
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 uint8_t *keys = s == 0 ? c.k + d.row * HD * ELEM : vt + row * STRIDE;
