@@ -327,7 +327,8 @@ struct Attend {
     float scale, cap;
     const float *slopes;
     int rows, tiles, columns;  // columns 0: a workgroup a row
-    int2 *meta;   // [row]: first and last slot
+    uint32_t least;            // of the plan
+    int2 *meta;   // [row]: first slot, segments
     float2 *ml;   // [slot][head]: reference (log2), sum
     float *sums;  // [slot][head][hd]
 };
@@ -413,51 +414,68 @@ __device__ __forceinline__ int64_t row_len(const Layer &c, const Attend &a, int6
     return pkv::clamp_len(a.k ? n + 1 : n, c.width, c.page);
 }
 
-// The segment of a slot, blocks b0 .. b1 - 1 of a row (none: b0 = b1 = 0);
-// every wave finds it by itself from the rows' lengths (a.rows <= kPlanRows).
+// Sums over a wave's lanes up to each (row_shr 1, 2, 4, 8, then the rows before).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+}
+
+// The segment of a slot: blocks b0 .. b1 - 1 of a row of `count` segments
+// (none: b0 = b1 = 0).  Every wave finds it by itself from the rows' lengths
+// (a.rows <= kPlanRows), a lane the same number of neighbouring rows.
 struct Part {
-    int row, b0, b1;
+    int row, b0, b1, count;
 };
 __device__ __forceinline__ Part find_part(const Layer &c, const Attend &a, uint32_t slot, int lane) {
     constexpr int N = pkv::kPlanRows / 64;
-    uint32_t nb[N], end[N], total = 0;
+    const int each = (a.rows + 63) >> 6;
+    uint32_t nb[N], segs[N], sum = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int r = 64 * i + lane;
+        if (i >= each) break;
+        const int r = lane * each + i;
         nb[i] = r < a.rows ? (uint32_t)((row_len(c, a, r) + B - 1) / B) : 0;
+        sum += nb[i];
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) {  // ends in the line of all blocks
-        end[i] = nb[i];
-        if (64 * i >= a.rows) break;
-        if (a.rows > 1)
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t up = __shfl_up(end[i], o);
-                if (lane >= o) end[i] += up;
-            }
-        end[i] += total;
-        total = __shfl(end[i], a.rows > 1 ? 63 : 0);
-    }
-    const uint32_t per = pkv::column_blocks(total, a.columns);
-    Part p{0, 0, 0};
+    const uint32_t per = pkv::per_of(__builtin_amdgcn_readlane(wave_scan(sum), 63), a.columns, a.least);
+    sum = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int r = 64 * i + lane;
-        p.row += __popcll(__ballot(r < a.rows && r + 1 + end[i] / per <= slot));
+        if (i >= each) break;
+        segs[i] = pkv::segments_of(nb[i], per);
+        sum += segs[i];
     }
-    if (p.row >= a.rows) return p;
-    uint32_t e = 0, n = 0;
+    const uint32_t end = wave_scan(sum);
+    const uint64_t who = __ballot(slot < end && slot >= end - sum);
+    Part p{0, 0, 0, 0};
+    if (who == 0) return p;
+    uint32_t left = slot - (end - sum), row = 0, n = 0, segments = 1, index = 0;
+    bool found = false;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const uint32_t x = __shfl(end[i], p.row & 63), y = __shfl(nb[i], p.row & 63);
-        if (i == p.row >> 6) e = x, n = y;
+        if (i >= each) break;
+        if (!found && left < segs[i]) {
+            found = true;
+            row = lane * each + i;
+            n = nb[i];
+            segments = segs[i];
+            index = left;
+        }
+        left -= segs[i];  // (not looked at once found)
     }
-    const uint64_t begin = e - n, column = (uint64_t)(slot - p.row) * per;
-    const uint64_t lo = column > begin ? column : begin, hi = e < column + per ? e : column + per;
-    if (lo >= hi) return p;
-    p.b0 = (int)(lo - begin);
-    p.b1 = (int)(hi - begin);
+    const int l = __ffsll((unsigned long long)who) - 1;
+    n = __builtin_amdgcn_readlane(n, l);
+    const uint32_t size = pkv::segment_blocks(n, __builtin_amdgcn_readlane(segments, l));
+    const uint32_t lo = __builtin_amdgcn_readlane(index, l) * size;
+    if (lo >= n) return p;
+    p.row = __builtin_amdgcn_readlane(row, l);
+    p.b0 = (int)lo;
+    p.b1 = (int)(n < lo + size ? n : lo + size);
+    p.count = (int)pkv::segments_of(n, size);
     return p;
 }
 
@@ -488,6 +506,13 @@ __device__ __forceinline__ int table_at(const int32_t *p) {
 // Each wave keeps its own and reads every fourth block; they are put
 // together through LDS.  A wave's next keys are on their way while it forms
 // the weights, its next values while it scores.
+//
+// Bound by reading the cache: 4 rows of 9001-32768 float16 positions, 8 heads
+// of 128 and 32 queries, 342 MB in 57.5 us (5.9 TB/s); 64 rows of 130-16384
+// int8, 1118 MB in 197 (5.7; a plain read of as many bytes 187).  One row of
+// 477 and 12 heads of 64 takes 8.3, a chain of loads: lengths and table, keys,
+// values.  Eight waves a workgroup were slower (75 and 254 us beside the 64
+// and 221 of four), as were blocks of 64 int8 positions (260 registers).
 template <int HD, int ELEM>
 __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c, Attend a) {
     constexpr int NT = B / 16, NC = HD * ELEM / 64, NF = HD / 32, ND = HD / 16, NV = 2 * ELEM;
@@ -502,14 +527,18 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     const int bpp = c.page / B;
     const bool low = n >= 8;
 
-    int64_t r = blockIdx.x;
-    int b0 = 0, b1 = 0;
+    const uint32_t slot = blockIdx.z * 8 + blockIdx.x;
+    int64_t r = slot;
+    int b0 = 0, b1 = 0, count = 0;
     if (a.columns) {
-        const Part part = find_part(c, a, blockIdx.x, lane);
+        const Part part = find_part(c, a, slot, lane);
         r = __builtin_amdgcn_readfirstlane(part.row);
         b0 = __builtin_amdgcn_readfirstlane(part.b0);
         b1 = __builtin_amdgcn_readfirstlane(part.b1);
+        count = __builtin_amdgcn_readfirstlane(part.count);
         if (b0 == b1) return;  // the same for the whole workgroup
+    } else if (r >= a.rows) {
+        return;
     }
     const int32_t *table = c.table + r * c.width;
     const int64_t told = (int64_t)a.len[r] + (a.k ? 1 : 0), len = uniform64(pkv::clamp_len(told, c.width, c.page));
@@ -824,10 +853,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
             if (q < 2) wsum[w][4 * q + i][16 * d + n] = ldexpf(fmaf(z, 0x1p-11f, y), ve - 8);
         }
     __syncthreads();
-    if (tid == 0 && blockIdx.y == 0 && a.columns) {
-        if (b0 == 0) a.meta[r].x = blockIdx.x;
-        if (b1 == nb) a.meta[r].y = blockIdx.x;
-    }
+    if (tid == 0 && blockIdx.y == 0 && a.columns && b0 == 0) a.meta[r] = make_int2(slot, count);
     for (int i = tid; i < hn * HD; i += 64 * pkv::kWaves) {
         const int h = i / HD, d = i % HD;
         float R = kLowest, L = 0.0f, o = 0.0f;
@@ -842,14 +868,16 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         if (whole) {
             a.out[r * a.ldo + (int64_t)(h0 + h) * HD + d] = L == 0.0f ? 0.0f : o / L;
         } else {
-            const int64_t slot = (int64_t)blockIdx.x * a.n_head + h0 + h;
-            a.sums[slot * HD + d] = o;
-            if (d == 0) a.ml[slot] = make_float2(R, L);
+            const int64_t at = (int64_t)slot * a.n_head + h0 + h;
+            a.sums[at * HD + d] = o;
+            if (d == 0) a.ml[at] = make_float2(R, L);
         }
     }
 }
 
-// The segments of a row put together, in their order: a workgroup a (head, row).
+// The segments of a row put together, in their order: a workgroup a (head,
+// row), all of a row's parts asked for at once up to 32.  5-6 us, of which the
+// launch is most: 4 x 32 of 65 parts 5.4, 64 x 32 of 1-4 parts 6.0.
 constexpr int kJoinWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Attend a) {
@@ -862,10 +890,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Atte
         if (threadIdx.x < HD) a.out[r * a.ldo + (int64_t)h * HD + threadIdx.x] = 0.0f;
         return;
     }
-    if (m.x == m.y) return;  // in one, which has written it
+    if (m.y == 1) return;  // in one, which has written it
     const float2 *ml = a.ml + (int64_t)m.x * a.n_head + h;
     const float *sums = a.sums + ((int64_t)m.x * a.n_head + h) * HD;
-    const int n = m.y - m.x + 1;
+    const int n = m.y;
     // a wave every fourth segment, kAtOnce of them asked for together
     constexpr int kAtOnce = 8;
     float R = kLowest, L = 0.0f, o[HD / 64] = {};
@@ -991,17 +1019,18 @@ int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, Atten
     a.meta = static_cast<int2 *>(work);
     a.ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(work) + at.ml);
     a.sums = reinterpret_cast<float *>(static_cast<uint8_t *>(work) + at.sums);
-    // rows that one column would take whole need no joining
-    const bool join = p.columns && width * kv->page > (int64_t)pkv::kMinBlocks * B;
+    const bool join = p.columns && width * (kv->page / B) > (int64_t)p.uncut;
     a.columns = join ? p.columns : 0;
-    // a multiple of the 8 XCDs: the tiles of one cached head land on one
-    const int64_t cols = join ? (pkv::slots_of(p, rows) + 7) / 8 * 8 : rows;
+    a.least = p.least;
+    // eight slots, one an XCD, of every head after one another: a slot's tiles share their XCD's L2, and the
+    // slots without a segment, the last, are the last to start
+    const int64_t slots = join ? pkv::slots_of(p, rows) : rows;
     LLMQ_REQUIRE(!join || rows * width * (kv->page / B) < pkv::kMaxBlocks, "%s: %lld table rows of %lld pages", name,
                  (long long)rows, (long long)width);
     return dispatch(kv, [&](auto hd, auto elem) -> int {
         hipLaunchKernelGGL((pkv_attend_kernel<decltype(hd)::value, decltype(elem)::value>),
-                           dim3((unsigned)cols, (unsigned)(kv->n_kv * p.tiles)), dim3(64 * pkv::kWaves), 0, ctx->stream,
-                           c, a);
+                           dim3(8, (unsigned)(kv->n_kv * p.tiles), (unsigned)((slots + 7) / 8)), dim3(64 * pkv::kWaves), 0,
+                           ctx->stream, c, a);
         if (join)
             hipLaunchKernelGGL((pkv_join_kernel<decltype(hd)::value>), dim3((unsigned)a.n_head, (unsigned)rows),
                                dim3(64 * kJoinWaves), 0, ctx->stream, c, a);
@@ -1116,7 +1145,7 @@ int64_t llmq_pkv_work_bytes(const llmq_pkv *kv, int64_t rows, int n_head) {
 int llmq_pkv_attend(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q, int64_t ldq,
                     int64_t rows, int n_head, const int32_t *len, const int32_t *table, int64_t width, float scale,
                     float cap, const float *slopes, void *work, int64_t work_bytes) {
-    Attend a{out, ldo, q, nullptr, nullptr, ldq, len, n_head, scale, cap, slopes, 0, 0, 0, nullptr, nullptr, nullptr};
+    Attend a{out, ldo, q, nullptr, nullptr, ldq, len, n_head, scale, cap, slopes, 0, 0, 0, 0, nullptr, nullptr, nullptr};
     return attend("pkv_attend", ctx, kv, layer, a, rows, table, width, work, work_bytes);
 }
 
@@ -1124,7 +1153,7 @@ int llmq_pkv_step(llmq_ctx *ctx, llmq_pkv *kv, int layer, float *out, int64_t ld
                   const float *v, int64_t ld, int64_t rows, int n_head, const int32_t *pos, const int32_t *table,
                   int64_t width, float scale, float cap, const float *slopes, void *work, int64_t work_bytes) {
     LLMQ_REQUIRE((k && v) || rows == 0, "pkv_step: null argument");
-    Attend a{out, ldo, q, k, v, ld, pos, n_head, scale, cap, slopes, 0, 0, 0, nullptr, nullptr, nullptr};
+    Attend a{out, ldo, q, k, v, ld, pos, n_head, scale, cap, slopes, 0, 0, 0, 0, nullptr, nullptr, nullptr};
     return attend("pkv_step", ctx, kv, layer, a, rows, table, width, work, work_bytes);
 }
 

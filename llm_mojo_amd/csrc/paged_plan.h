@@ -39,42 +39,60 @@ PKV_HD int64_t clamp_len(int64_t len, int64_t width, int page) {
 
 // How a call's rows are split over workgroups.  A workgroup takes up to 8 of
 // the query heads of a cached head (`tiles` of them cover the group).  Up to
-// kPlanRows rows, the blocks of all rows in one line are cut into columns of
-// one size, and a workgroup takes what a column has of a row (a segment): a
-// long row gets many, a short one one.  More rows fill the card by
-// themselves: a workgroup a row (columns 0).
+// kPlanRows rows, a row of more than `per` blocks (per_of, from the sum over
+// all rows) is cut into segments of one size, each a workgroup; the segments
+// of all rows, one after another, are the slots of the grid and of the
+// workspace.  More rows fill the card by themselves: a workgroup a row
+// (columns 0), as do tables of `uncut` blocks at most, whose rows end before a
+// second launch would have joined their parts.
+//
+// kWorkgroups: 2.7 times those that run at once.  4 rows of float16, 342 MB:
+// 1536 64.9 us, 2048 62.2, 3072 65; 64 rows of int8, 1082 MB: 199, 201, 204.
+// kPlanRows: 300 rows of up to 16384 positions and one head, each its own
+// workgroup 255 us, cut 139; 600 rows 203 and 151.
 constexpr int kWaves = 4;         // of a workgroup, each taking every kWaves-th block
-constexpr int kMinBlocks = 16;    // of a column
-constexpr int kPlanRows = 256;    // rows whose lengths a wave holds at once
+constexpr int kPlanRows = 1024;   // rows whose lengths a wave holds at once
 constexpr int kWorkgroups = 2048;
-constexpr int64_t kMaxBlocks = (int64_t)1 << 31;  // of all rows' tables, where they are cut into columns
+constexpr int64_t kMaxBlocks = (int64_t)1 << 31;  // of all rows' tables, where they may be cut
+
+// Where rows and heads give each CU a workgroup, rows are cut later: 32 rows x
+// 8 heads of 1000 positions whole 19.4 us, in segments of 8 blocks 25.8, and
+// of 2000 in a table for as many, uncut 26.6, cut 31.4.  With fewer: 4 x 8
+// heads of up to 2000, segments of at least 8 blocks 17.1, 16 18.7, uncut 22.
+constexpr int kCUs = 256;
 
 struct Plan {
     int tiles, columns;
+    uint32_t least, uncut;  // blocks of a row, and of a table, that is not cut
 };
 
 PKV_HD Plan plan_of(int64_t rows, int n_head, int n_kv) {
     Plan p;
     p.tiles = (n_head / n_kv + 7) / 8;
-    p.columns = 0;
-    if (rows > kPlanRows) return p;
     const int64_t all = (int64_t)n_kv * p.tiles;
-    p.columns = all >= kWorkgroups ? 1 : (int)(kWorkgroups / all);
+    const bool many = rows * all >= kCUs;
+    p.columns = rows > kPlanRows ? 0 : (all >= kWorkgroups ? 1 : (int)(kWorkgroups / all));
+    p.least = many ? 32 : 8;
+    p.uncut = many ? 64 : 32;
     return p;
 }
 
-// Blocks of a column, given those of all rows: at most `columns` columns, a multiple of the waves.
-PKV_HD uint32_t column_blocks(uint32_t total, int columns) {
+// Blocks of a segment at most, given those of all rows.
+PKV_HD uint32_t per_of(uint32_t total, int columns, uint32_t least) {
     const uint32_t n = total / (uint32_t)columns + 1;
-    return n < (uint32_t)kMinBlocks ? (uint32_t)kMinBlocks : (n + kWaves - 1) / kWaves * kWaves;
+    return n < least ? least : (n + kWaves - 1) / kWaves * kWaves;
+}
+// Segments of a row, and their blocks (the last one's may be fewer): a multiple of the waves, so a row may
+// need fewer of them than it has slots.
+PKV_HD uint32_t segments_of(uint32_t blocks, uint32_t per) { return (blocks + per - 1) / per; }
+PKV_HD uint32_t segment_blocks(uint32_t blocks, uint32_t segments) {
+    return ((blocks + segments - 1) / segments + kWaves - 1) / kWaves * kWaves;
 }
 
-// Row r, whose blocks are [begin, end) of the line, has its segments of columns begin / per ... in slots
-// r + column: the pairs of (row, column) go up in one or both along the line, so no two share a slot, and
-// the row of a slot is the number of rows k with k + 1 + end of k / per at most the slot.
+// Slots at most: a segment a row, and one a column, since per is above total / columns.
 PKV_HD int64_t slots_of(const Plan &p, int64_t rows) { return p.columns ? p.columns + rows : 0; }
 
-// Byte offsets of a call's workspace: per row its first and last column, per
+// Byte offsets of a call's workspace: per row its first slot and its segments, per
 // (slot, head) the reference and sum of its exponentials, and its sums of values.
 struct Work {
     int64_t ml, sums, bytes;

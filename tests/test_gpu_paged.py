@@ -291,6 +291,49 @@ def test_attend_many_rows(gpu, kind):
     check(c, 4)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 128, 129, 700, 1024, 1025])
+@pytest.mark.parametrize("kind", KINDS)
+def test_attend_rows_cut_into_segments(gpu, kind, rows):
+    """Tables for more than a row that is never cut, at the edges of the rows
+    that a lane and the plan hold: short rows, empty ones and a few long ones,
+    whose segments are joined."""
+    rng = np.random.default_rng(rows)
+    for heads, n_kv in ((8, 1), (18, 2)):
+        print("segments", kind, rows, heads, flush=True)
+        lens = rng.integers(0, 70, rows)
+        lens[rng.random(rows) < 0.1] = 0
+        for n in (2500, 1057, 3001, 300)[:rows]:
+            lens[rng.integers(0, rows)] = n
+        c = Case(gpu, kind, 64, n_kv, [int(x) for x in lens], width=50)
+        check(c, heads)
+        c.cache.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_step_rows_cut_into_segments(gpu, kind):
+    """Steps whose new token is in a segment's first, last and only block, and attend after them."""
+    torch, lm, ctx = gpu
+    lens = [2048, 2047, 1, 33, 511, 512, 513, 1024, 0, 1999]
+    c = Case(gpu, kind, 128, 2, [n + 1 for n in lens], width=40)
+    n, heads = len(lens), 18
+    x = dev(torch, c.rng.normal(0, 1, (n, heads + 4, 128)).astype(np.float32))
+    pos = dev(torch, np.array(lens, np.int32))
+    out, again = (torch.full((n, heads, 128), float("nan"), device="cuda") for _ in range(2))
+    w, _ = c.work(n, heads)
+    c.cache.step(0, out, x[:, :heads], x[:, heads:heads + 2], x[:, heads + 2:], pos, c.table, w)
+    c.cache.attend(0, again, x[:, :heads], pos + 1, c.table, w)
+    for r, p in enumerate(lens):
+        at = [torch.full((p + 1,), r, dtype=torch.int32, device="cuda"),
+              torch.arange(p + 1, dtype=torch.int32, device="cuda")]
+        k, v = (torch.empty(p + 1, 2, 128, device="cuda") for _ in range(2))
+        c.cache.fetch(0, k, v, *at, c.table)
+        k, v = k.cpu().numpy(), v.cpu().numpy()
+        assert np.array_equal(k[p], held(kind, x[r, heads:heads + 2].cpu().numpy()))
+        o, bar = want(x[r, :heads].cpu().numpy(), k, v, 1 / math.sqrt(128), 0.0, None)
+        for y in (out, again):
+            assert np.all(np.abs(y[r].cpu().numpy() - o) <= bar), r
+
+
 @pytest.mark.parametrize("cap,bias,scale", [(30.0, False, None), (0.0, True, None), (5.0, True, 0.3), (0.0, False, 1e-9),
                                             (0.0, False, -0.125), (0.0, False, 3.0)])
 @pytest.mark.parametrize("kind", KINDS)

@@ -17,12 +17,15 @@ int value_slot(int p) { return pkv::value_slot(p); }
 int page_of(const int32_t *row, int64_t w, int page, int64_t pages, int64_t pos) {
     return pkv::page_of(row, w, page, pages, pos); }
 int64_t clamp_len(int64_t n, int64_t w, int page) { return pkv::clamp_len(n, w, page); }
-void plan(int64_t rows, int n_head, int n_kv, int hd, int64_t *out) {
+void plan(int64_t rows, int n_head, int n_kv, int hd, int64_t *out) {  // 7 numbers
     const pkv::Plan p = pkv::plan_of(rows, n_head, n_kv);
     const pkv::Work w = pkv::work_of(p, rows, n_head, hd);
     out[0] = p.tiles; out[1] = p.columns; out[2] = pkv::slots_of(p, rows); out[3] = w.ml; out[4] = w.sums; out[5] = w.bytes;
+    out[6] = p.least;
 }
-uint32_t column_blocks(uint32_t total, int columns) { return pkv::column_blocks(total, columns); }
+uint32_t per_of(uint32_t total, int columns, uint32_t least) { return pkv::per_of(total, columns, least); }
+uint32_t segments_of(uint32_t blocks, uint32_t per) { return pkv::segments_of(blocks, per); }
+uint32_t segment_blocks(uint32_t blocks, uint32_t segments) { return pkv::segment_blocks(blocks, segments); }
 }
 """
 
@@ -38,7 +41,10 @@ def plan(tmp_path_factory):
     i64 = ctypes.c_int64
     L.page_of.argtypes = [ctypes.c_void_p, i64, ctypes.c_int, i64, i64]
     L.plan.argtypes = [i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
-    L.column_blocks.argtypes, L.column_blocks.restype = [ctypes.c_uint32, ctypes.c_int], ctypes.c_uint32
+    u32 = ctypes.c_uint32
+    L.per_of.argtypes, L.per_of.restype = [u32, ctypes.c_int, u32], u32
+    L.segments_of.argtypes, L.segments_of.restype = [u32, u32], u32
+    L.segment_blocks.argtypes, L.segment_blocks.restype = [u32, u32], u32
     L.clamp_len.argtypes, L.clamp_len.restype = [i64, i64, ctypes.c_int], i64
     return L
 
@@ -82,36 +88,36 @@ def blocks(rng, rows):
     return nb
 
 
-def test_columns_cover_the_rows_and_fit(plan):
-    """Any lengths: every block is in one slot's segment, found from the slot
-    as the kernel does, and the slots fit the grid and the workspace."""
+def test_segments_cover_the_rows_and_fit(plan):
+    """Any lengths: a row's segments cover its blocks, and the slots of all rows fit the grid and the workspace."""
     rng = np.random.default_rng(1)
-    out = np.zeros(6, np.int64)
+    out = np.zeros(7, np.int64)
     for _ in range(1500):
-        rows = int(2 ** rng.uniform(0, 8))
+        rows = int(2 ** rng.uniform(0, 10))
         n_kv = int(rng.choice([1, 2, 3, 4, 8, 12, 32, 129, 600, 2000]))
         n_head = n_kv * int(rng.choice([1, 2, 7, 8, 9, 16, 71]))
         hd = int(rng.choice([64, 128]))
         plan.plan(rows, n_head, n_kv, hd, out.ctypes.data)
-        tiles, columns, slots, ml, sums, size = (int(x) for x in out)
+        tiles, columns, slots, ml, sums, size, least = (int(x) for x in out)
         assert tiles * 8 >= n_head // n_kv > (tiles - 1) * 8
         assert columns >= 1 and (columns == 1 or n_kv * tiles * columns <= 2048) and slots == rows + columns
         assert ml >= rows * 8 and sums >= ml + slots * n_head * 8 and size == sums + slots * n_head * hd * 4
         assert ml % 256 == 0 and sums % 256 == 0
         nb = blocks(rng, rows)
-        total = int(nb.sum())
-        per = plan.column_blocks(total, columns)
-        assert per >= 16 and per % 4 == 0 and -(-total // per) <= columns and per <= 2 ** 31
-        ends = np.cumsum(nb)
-        covered = np.zeros(rows, np.int64)
-        for s in range(slots):
-            r = int((np.arange(rows) + 1 + ends // per <= s).sum())
-            j = s - r
-            if r >= rows or j < 0:
+        per = plan.per_of(int(nb.sum()), columns, least)
+        assert per >= least >= 8 and per % 4 == 0 and per <= 2 ** 31
+        used = 0
+        for n in (int(x) for x in nb):
+            segments = plan.segments_of(n, per)
+            used += segments
+            assert segments == -(-n // per)
+            if n == 0:
                 continue
-            lo, hi = max(j * per, ends[r] - nb[r]), min((j + 1) * per, ends[r])
-            if lo < hi:
-                covered[r] += hi - lo
-        assert (covered == nb).all()
-    plan.plan(257, 12, 12, 64, out.ctypes.data)
+            seg = plan.segment_blocks(n, segments)
+            count = plan.segments_of(n, seg)
+            assert seg % 4 == 0 and 1 <= count <= segments and (segments - 1) * seg < 2 ** 32
+            assert (count - 1) * seg < n <= count * seg  # the slots from count on are empty
+            assert n > least or segments == 1
+        assert used <= slots
+    plan.plan(1025, 12, 12, 64, out.ctypes.data)
     assert out[1] == 0 and out[2] == 0 and out[5] == out[4]
