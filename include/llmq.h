@@ -375,7 +375,9 @@ LLMQ_API int llmq_pkv_attend(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float
 /* A decode step's attention: row r's new key and value (rows of k and v, ld
  * apart like q's) are stored at position pos[r] of table row r, then its
  * query heads attend to positions 0 .. pos[r].  pos[r] < 0: no token, zeros.
- * No row of a call may attend to a position that another row of it stores. */
+ * No row of a call may attend to a position that another row of it stores,
+ * or to the one it stores under two places of its table row.  out is apart
+ * from q, k and v. */
 LLMQ_API int llmq_pkv_step(llmq_ctx *ctx, llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q,
                            const float *k, const float *v, int64_t ld, int64_t rows, int n_head, const int32_t *pos,
                            const int32_t *table, int64_t width, float scale, float cap, const float *slopes,

@@ -183,7 +183,9 @@ struct Floats4 {
     float x[4];
 } __attribute__((packed, aligned(4)));
 
-// llmq_pkv_store.
+// llmq_pkv_store.  Bound by reading the floats and writing the cache: 17.7k
+// positions x 8 x 128 to float16 49 us (218 MB, 4.4 TB/s; 62 with plain loads),
+// 476 x 12 x 64 to int8 5.
 template <int HD, int ELEM>
 __global__ __launch_bounds__(kRows *kLanes) void pkv_store_kernel(Layer c, const float *__restrict__ k,
                                                                   const float *__restrict__ v, int64_t ld, int64_t T,
@@ -253,7 +255,8 @@ __global__ __launch_bounds__(kRows *kLanes) void pkv_store_kernel(Layer c, const
     }
 }
 
-// llmq_pkv_fetch; zeros where the cache has no row.
+// llmq_pkv_fetch; zeros where the cache has no row.  The same rows back: 39 us
+// (5.5 TB/s) and 4.3.
 template <int HD, int ELEM>
 __global__ __launch_bounds__(kRows *kLanes) void pkv_fetch_kernel(Layer c, float *__restrict__ k,
                                                                   float *__restrict__ v, int64_t ld, int64_t T,
