@@ -359,7 +359,7 @@ LLMQ_API int llmq_pkv_fetch(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float 
 /* Attention of one token a sequence: row r's n_head query heads (device
  * floats, rows ldq apart) over positions 0 .. len[r] - 1 of table row r,
  * query head h over cached head h / (n_head / n_kv):
- *   s_j = scale q . k_j;  s_j = cap tanh(s_j / cap) when cap > 0;
+ *   s_j = scale q . k_j;  s_j = cap tanh(s_j / cap) when cap > 0 (normal);
  *   s_j += slopes[h] (j - (len[r] - 1)) when slopes is given;
  *   out = sum_j softmax(s)_j v_j.
  * A length of 0 (or less) gives zeros; lengths past the table's row end with

@@ -1006,7 +1006,8 @@ int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, Atten
     const int64_t need = (int64_t)a.n_head * kv->hd;
     LLMQ_REQUIRE(a.ldo >= need && a.ldq >= need, "%s: row strides %lld, %lld below %lld", name, (long long)a.ldo,
                  (long long)a.ldq, (long long)need);
-    LLMQ_REQUIRE(a.scale == a.scale && a.cap >= 0.0f && a.cap <= 3.0e38f, "%s: scale %g, cap %g", name, a.scale, a.cap);
+    LLMQ_REQUIRE(a.scale == a.scale && (a.cap == 0.0f || (a.cap >= 1.2e-38f && a.cap <= 3.0e38f)),
+                 "%s: scale %g, cap %g", name, a.scale, a.cap);  // (1 / cap is finite)
     const int64_t want = llmq_pkv_work_bytes(kv, rows, a.n_head);
     LLMQ_REQUIRE(work_bytes >= want, "%s: %lld bytes of work, %lld needed", name, (long long)work_bytes,
                  (long long)want);

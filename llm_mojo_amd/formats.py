@@ -244,10 +244,20 @@ class HipMX4Matrix:
             pass
 
 
+_dtypes = {}  # the names of tensors' types, which take half a microsecond each to form
+
+
+def _is(t, name):
+    n = _dtypes.get(t.dtype)
+    if n is None:
+        n = _dtypes[t.dtype] = str(t.dtype)
+    return n == name
+
+
 def _mx4_rows(ctx, x, codes, scales):
     """(rows, columns, row stride) of x[T, K] with packed codes[T, K / 2] and scales[T, K / 32]."""
     T, K = x.shape
-    if str(x.dtype) != "torch.float32" or x.get_device() != ctx.device or (x.numel() and x.stride(1) != 1):
+    if not _is(x, "torch.float32") or x.get_device() != ctx.device or (x.numel() and x.stride(1) != 1):
         raise ValueError(f"mx4: float32 rows in one piece on GPU {ctx.device}")
     _mx4_packed(ctx, codes, scales, T, K)
     return T, K, x.stride(0) if T > 1 else max(x.stride(0), K)
@@ -255,8 +265,7 @@ def _mx4_rows(ctx, x, codes, scales):
 
 def _mx4_packed(ctx, codes, scales, T, K):
     for t, shape in ((codes, (T, K // 2)), (scales, (T, K // 32))):
-        if (str(t.dtype) != "torch.uint8" or t.get_device() != ctx.device or not t.is_contiguous()
-                or tuple(t.shape) != shape):
+        if not _is(t, "torch.uint8") or t.get_device() != ctx.device or not t.is_contiguous() or t.shape != shape:
             raise ValueError(f"mx4: contiguous uint8 codes [{T}, {K // 2}] and scales [{T}, {K // 32}] on GPU "
                              f"{ctx.device}")
 
@@ -277,7 +286,7 @@ def mx4_linear(ctx, out, codes, scales, w, bias=None, resid=False, gelu=False):
     """linear over rows that mx4_quantize left: out (+)= act(x @ w^T + bias)."""
     _mx4_packed(ctx, codes, scales, codes.shape[0], w.cols)
     for t, shape in ((out, (codes.shape[0], w.rows)), (bias, (w.rows,))):
-        if t is not None and (str(t.dtype) != "torch.float32" or not t.is_contiguous() or tuple(t.shape) != shape
+        if t is not None and (not _is(t, "torch.float32") or not t.is_contiguous() or t.shape != shape
                               or t.get_device() != ctx.device):
             raise ValueError(f"mx4_linear: a contiguous float32 out[{codes.shape[0]}, {w.rows}] and bias[{w.rows}] on "
                              f"GPU {ctx.device}")

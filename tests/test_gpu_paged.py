@@ -531,6 +531,43 @@ def test_step_in_a_graph(gpu, kind):
         assert torch.equal(out, ob), i
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_store_and_fetch_in_a_graph(gpu, kind):
+    """A captured store and fetch take the rows, positions and tables that are there at each replay."""
+    torch, lm, ctx = gpu
+    rng = np.random.default_rng(4)
+    c = lm.PagedKV(ctx, 1, 12, 64, 2, 64, kind)
+    T = 70
+    k, v, ko, vo = (torch.zeros(T, 2, 64, device="cuda") for _ in range(4))
+    seq, pos = (torch.zeros(T, dtype=torch.int32, device="cuda") for _ in range(2))
+    table = torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(side):
+            ctx.set_stream(side)
+            graph.capture_begin()
+            c.store(0, k, v, seq, pos, table)
+            c.fetch(0, ko, vo, seq, pos, table)
+            graph.capture_end()
+    finally:
+        ctx.set_stream(torch.cuda.current_stream())
+    for i in range(5):
+        table.copy_(dev(torch, rng.permutation(12).reshape(3, 4).astype(np.int32)))
+        s, first = rng.integers(0, 3), rng.integers(0, 180)
+        seq.fill_(int(s))
+        pos.copy_(torch.arange(T, dtype=torch.int32) + int(first))
+        x, y = (rng.normal(0, 1, (T, 2, 64)).astype(np.float32) for _ in range(2))
+        k.copy_(dev(torch, x))
+        v.copy_(dev(torch, y))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(ko.cpu().numpy(), held(kind, x)) and np.array_equal(vo.cpu().numpy(), held(kind, y)), i
+
+
 def test_streams(gpu):
     """Two caches on two streams, and a context moved between them."""
     torch, lm, ctx = gpu
@@ -575,6 +612,7 @@ def test_refusals(gpu):
         lambda: c.attend(0, out, q, ln, table, w[:-1]),
         lambda: c.attend(0, out, q, ln, table, w, cap=-1.0),
         lambda: c.attend(0, out, q, ln, table, w, cap=float("nan")),
+        lambda: c.attend(0, out, q, ln, table, w, cap=1e-40),
         lambda: c.attend(0, out, q, ln, table, w, scale=float("nan")),
         lambda: c.attend(0, out, q, ln, table, w, slopes=z(3)),
         lambda: c.attend(0, out, q.cpu(), ln, table, w),
