@@ -237,12 +237,43 @@ __global__ __launch_bounds__(256) void mx4_weights_kernel(const float *__restric
     scales[((tile * words + (step >> 2)) * 64 + lane) * 4 + (step & 3)] = (uint8_t)e;
 }
 
+// GELU in its tanh form, 0.5 r (1 + tanh z) = r / (1 + e^-2z) with z =
+// sqrt(2 / pi) (r + 0.044715 r^3): one exponential and a reciprocal, no branches
+// and no cancellation for negative r.
+__device__ __forceinline__ float gelu_of(float r) {
+    const float u = fmaf(0.044715f * r * r, r, r);
+    const float e = __builtin_amdgcn_exp2f(u * -2.302208198f);  // -2 sqrt(2 / pi) log2 e
+    return r * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 // act(sum + bias) (+ what is there): the epilogue of every product here.
 __device__ __forceinline__ void finish(float *p, float y, const float *bias, int64_t o, int flags) {
     if (flags & LLMQ_BIAS) y = y + bias[o];
-    if (flags & LLMQ_GELU) y = gelu_ref(y);
+    if (flags & LLMQ_GELU) y = gelu_of(y);
     if (flags & LLMQ_RESID) y = *p + y;
     *p = y;
+}
+
+// Four of a row's n floats from o on, zeros past its end, and back.
+__device__ __forceinline__ v4f load_four(const float *p, int o, int n) {
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (o + 4 <= n) {
+        v = __builtin_bit_cast(v4f, *reinterpret_cast<const Float4 *>(p + o));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (o + i < n) v[i] = p[o + i];
+    }
+    return v;
+}
+__device__ __forceinline__ void store_four(float *p, const v4f &v, int o, int n) {
+    if (o + 4 <= n) {
+        *reinterpret_cast<Float4 *>(p + o) = __builtin_bit_cast(Float4, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (o + i < n) p[o + i] = v[i];
+    }
 }
 
 // Operands of a product: tokens in packed rows (codes K / 2 and scales K / 32
@@ -566,28 +597,38 @@ __global__ __launch_bounds__(256, 2) void mx4_many_kernel(Product p, int gx, int
     }
     if (g < groups) group(g, c0, c1, s0, s1);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): no copy into LDS is left behind
-    const bool wide = p.n % 4 == 0 && (uintptr_t)p.out % 16 == 0 && !(p.flags & ~LLMQ_BIAS);
+    // Four outputs a load and a store, whatever their alignment: 2048 x 4096 x 11008 with GELU 67 us, with bias and
+    // residual 75; an output at a time they took 106 and 155, and 1024 x 4096 x 11009 53 for 37.  (The waves of the
+    // matrix's last outputs look at each four.)
+    auto write = [&](auto whole) __attribute__((always_inline)) {
+        const int n = decltype(whole)::value ? INT32_MAX : p.n;
+        v4f bias[4] = {};
+        if (p.flags & LLMQ_BIAS)
 #pragma unroll
-    for (int t = 0; t < TT; t++) {
-        if (16 * t + c >= live) continue;
-        float *row = p.out + (t0 + 16 * t + c) * p.n;
+            for (int r = 0; r < 4; r++) bias[r] = load_four(p.bias, (tile0 + r) * 16 + 4 * q, n);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int o = (tile0 + r) * 16 + 4 * q;
-            if (wide) {
-                if (o >= p.n) continue;
-                v4f y = acc[r][t];
-                if (p.flags & LLMQ_BIAS)
+        for (int t = 0; t < TT; t++) {
+            if (16 * t + c >= live) continue;
+            float *row = p.out + (t0 + 16 * t + c) * p.n;
+            v4f there[4];
+            if (p.flags & LLMQ_RESID)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) y[i] += p.bias[o + i];
-                *reinterpret_cast<v4f *>(row + o) = y;
-            } else {
+                for (int r = 0; r < 4; r++) there[r] = load_four(row, (tile0 + r) * 16 + 4 * q, n);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (o + i < p.n) finish(row + o + i, acc[r][t][i], p.bias, o + i, p.flags);
+            for (int r = 0; r < 4; r++) {
+                v4f y = acc[r][t] + bias[r];
+                if (p.flags & LLMQ_GELU)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[i] = gelu_of(y[i]);
+                if (p.flags & LLMQ_RESID) y = there[r] + y;
+                store_four(row, y, (tile0 + r) * 16 + 4 * q, n);
             }
         }
-    }
+    };
+    if ((tile0 + 4) * 16 <= p.n)
+        write(std::true_type{});
+    else
+        write(std::false_type{});
 }
 
 int check_shape(const char *name, int64_t rows, int64_t cols) {
@@ -695,18 +736,22 @@ int launch_many(llmq_ctx *ctx, const Product &p) {
     return LLMQ_OK;
 }
 
-// The kernel by the number of workgroups.  Few-token workgroups cost the
-// same each, however many there are, the others fill the CUs with few: up to
-// 1280 of the first are the faster (2048 outputs: 256 tokens 10.9 us against
-// 17; 11008 outputs: 128 tokens 16.4 against 14.8).  Of the two large tiles
-// the one whose workgroups, a CU's share of them after one another, are done
-// first: 2048 x 4096 x 11008 68 us with 96 tokens, 75.5 with 64; 2048 x 11008 x
-// 4096 75 and 69.
+// The kernel by its time, whichever way the tokens are given (their sums are
+// then in one order).  Few-token workgroups cost the same each, 1.5 to 3 ns a
+// group of 512 inputs, however many there are; the others fill the CUs with few,
+// a chain of 1.4 us a group behind 5.5 us.  300 x 4096 x 4096 30.6 us by the
+// first and 17.1 by the others, 500 x 1024 x 1024 6.0 and 8.3, 32 x 4096 x 32000
+// 25 and 16, 40 x 4096 x 11008 16.1 and 13.7 (a record 10.7 and 13.9): over 280
+// sizes of 40 to 500 tokens 0.9 % behind the better of the two in the mean.  Of
+// the two large tiles the one whose workgroups, a CU's share of them after one
+// another, are done first: 2048 x 4096 x 11008 68 us with 96 tokens, 75.5 with
+// 64; 2048 x 11008 x 4096 75 and 69.
 template <int X>
 int launch_tokens(llmq_ctx *ctx, const Product &p, const llmq_mat *w) {
+    const int64_t work = w->ntiles * w->NG, bound = 650 * (w->NG + 3);
     if (p.T <= 16) return launch_few<1, X>(ctx, p, w, 0);
-    if (p.T <= 32) return launch_few<2, X>(ctx, p, w, 0);
-    if (w->ntiles * ((p.T + 63) / 64) <= 1280) return launch_few<4, X>(ctx, p, w, 0);
+    if (p.T <= 32 && 2 * work <= 3 * bound) return launch_few<2, X>(ctx, p, w, 0);
+    if (work * ((p.T + 63) / 64) <= bound) return launch_few<4, X>(ctx, p, w, 0);
     const int64_t gx = (w->n + kOuts - 1) / kOuts;
     auto cost = [&](int64_t tt) { return (gx * ((p.T + 16 * tt - 1) / (16 * tt)) + 255) / 256 * (5 * tt + 6); };
     return cost(6) < cost(4) ? launch_many<6, X>(ctx, p) : launch_many<4, X>(ctx, p);
