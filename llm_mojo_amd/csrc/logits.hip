@@ -85,8 +85,9 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
     constexpr int N = CHUNK / (4 * kThreads);  // fours of entries a thread
     __shared__ __align__(16) int count[CHUNK];
     __shared__ __align__(16) float add[CHUNK];
-    __shared__ int ids[kThreads], from[kThreads / 64];
-    __shared__ float val[kThreads];
+    __shared__ __align__(16) int ids[kThreads + 4];  // (a batch's, then -1)
+    __shared__ int from[kThreads / 64];
+    __shared__ __align__(16) float val[kThreads + 4];
     __shared__ Best red[kThreads / 64];
     const int64_t r = blockIdx.y;
     const int v0 = blockIdx.x * CHUNK, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -160,17 +161,25 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
                 ids[k] = (int)at;
                 val[k] = b;
             }
+            if (tid < 4) ids[n + tid] = -1;
             __syncthreads();
             if (tid < n) {
                 const int mine = ids[tid];
-                bool lead = true;
-                for (int k = 0; k < tid; k++) lead &= ids[k] != mine;
-                if (lead) {
-                    float s = add[mine];
-                    for (int k = tid; k < n; k++)
-                        if (ids[k] == mine) s += val[k];
-                    add[mine] = s;
+                int lead = -1;
+                float s = add[mine];
+                for (int k = 0; k < n; k += 4) {  // (the same for all lanes: four reads in one)
+                    const int4 id = *reinterpret_cast<const int4 *>(ids + k);
+                    const float4 b4 = *reinterpret_cast<const float4 *>(val + k);
+                    const int is[4] = {id.x, id.y, id.z, id.w};
+                    const float bs[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const bool same = is[j] == mine;
+                        lead = same && lead < 0 ? k + j : lead;
+                        s = same ? s + bs[j] : s;
+                    }
                 }
+                if (lead == tid) add[mine] = s;
             }
             __syncthreads();
         }
