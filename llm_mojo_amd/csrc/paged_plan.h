@@ -55,10 +55,12 @@ constexpr int kPlanRows = 1024;   // rows whose lengths a wave holds at once
 constexpr int kWorkgroups = 2048;
 constexpr int64_t kMaxBlocks = (int64_t)1 << 31;  // of all rows' tables, where they may be cut
 
-// Where rows and heads give each CU a workgroup, rows are cut later: 32 rows x
-// 8 heads of 1000 positions whole 19.4 us, in segments of 8 blocks 25.8, and
-// of 2000 in a table for as many, uncut 26.6, cut 31.4.  With fewer: 4 x 8
-// heads of up to 2000, segments of at least 8 blocks 17.1, 16 18.7, uncut 22.
+// A segment's least blocks, by how many of the CUs rows and heads alone give a
+// workgroup, and twice as many in a table that is not cut.  In a graph, us:
+// 1 row x 8 heads of 900 float16 positions cut into 8 blocks 11.8, uncut 17.7, of
+// 500 12.2 and 11.6; 16 x 8 of 1000 int8 uncut 14.8, cut 16.4, of 2000 in 16
+// blocks 20.3, in 8 25; 32 x 8 of 1000 uncut 16.1, in 16 21, and in a table for
+// 4096 whole 19.4, in 8 25.8.
 constexpr int kCUs = 256;
 
 struct Plan {
@@ -70,10 +72,9 @@ PKV_HD Plan plan_of(int64_t rows, int n_head, int n_kv) {
     Plan p;
     p.tiles = (n_head / n_kv + 7) / 8;
     const int64_t all = (int64_t)n_kv * p.tiles;
-    const bool many = rows * all >= kCUs;
     p.columns = rows > kPlanRows ? 0 : (all >= kWorkgroups ? 1 : (int)(kWorkgroups / all));
-    p.least = many ? 32 : 8;
-    p.uncut = many ? 64 : 32;
+    p.least = rows * all >= kCUs ? 32 : (rows * all >= kCUs / 2 ? 16 : 8);
+    p.uncut = 2 * p.least;
     return p;
 }
 
