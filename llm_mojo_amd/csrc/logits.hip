@@ -8,7 +8,7 @@
 // adds: the order does not matter), so no table of counts goes through
 // memory; a history is read once a chunk, from the caches after the first.
 // 256 rows x 50257 with histories of up to 2048 tokens, 64 biases and a mask
-// take 29.6 us (106 MB, 3.6 TB/s), one row x 32000 5.2.
+// take 28.9 us (106 MB, 3.7 TB/s), one row x 32000 5.2.
 //
 // Chunks of 2048 entries: 4096 took 37 us there, 512 threads 36.  Of 1024
 // where larger ones would leave CUs without a workgroup.
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const float *in
     if (tid == 0) parts[r * gridDim.x + blockIdx.x] = b;
 }
 
-// A row's chunks' picks put together: a wave a row (4.6 us for 256 rows of 25, most of it the launch).
+// A row's chunks' picks put together: a wave a row (4 us for 256 rows of 25, most of it the launch).
 __global__ __launch_bounds__(64) void pick_kernel(const Best *__restrict__ parts, int n, int64_t *__restrict__ pick) {
     const Best *p = parts + (int64_t)blockIdx.x * n;
     Best b{-INFINITY, INT32_MAX};

@@ -447,9 +447,10 @@ __global__ __launch_bounds__(64 * few_most(TT)) void mx4_few_kernel(Product p, i
 // the 1 KB that a wave reads of it, without passing through registers; their
 // scales are put into words there a group ahead.  A wave's weights, which no
 // other wave of the workgroup reads, come straight to its registers three
-// steps ahead, 1 KB in one piece.  With the loads, copies, barriers and LDS
-// reads left out, 2048 x 4096 x 11008 still takes 38 us of the 58 that the
-// kernel takes: 18 of products (16 cycles each), the rest its 90 MB of outputs.  Tiles
+// steps ahead, 1 KB in one piece.  2048 x 4096 x 11008 takes 67 us
+// (2750 TFLOP/s): the products 20 on full CUs (16 cycles each), its 90 MB of
+// outputs 13 behind them, prologues, copies and barriers the rest; eight waves on
+// twice the tokens, which read a third less from L2, took as long.  Tiles
 // of 128 tokens need more than 256 registers.
 constexpr int kOuts = 256;
 template <int TT, int X>

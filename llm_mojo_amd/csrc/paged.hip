@@ -518,7 +518,7 @@ __device__ __forceinline__ int table_at(const int32_t *p) {
 //
 // Bound by reading the cache: 4 rows of 9001-32768 float16 positions, 8 heads
 // of 128 and 32 queries, 342 MB in 57.5 us (5.9 TB/s); 64 rows of 130-16384
-// int8, 1118 MB in 197 (5.7; a plain read of as many bytes 187).  One row of
+// int8, 1118 MB in 198 (5.6; a plain read of as many bytes 187).  One row of
 // 477 and 12 heads of 64 takes 8.3, a chain of loads: lengths and table, keys,
 // values.  Eight waves a workgroup were slower (75 and 254 us beside the 64
 // and 221 of four), as were blocks of 64 int8 positions (260 registers).
