@@ -1038,9 +1038,9 @@ int attend(const char *name, llmq_ctx *ctx, const llmq_pkv *kv, int layer, Atten
     LLMQ_REQUIRE(!join || rows * width * (kv->page / B) < pkv::kMaxBlocks, "%s: %lld table rows of %lld pages", name,
                  (long long)rows, (long long)width);
     return dispatch(kv, [&](auto hd, auto elem) -> int {
-        hipLaunchKernelGGL((pkv_attend_kernel<decltype(hd)::value, decltype(elem)::value>),
-                           dim3(8, (unsigned)(kv->n_kv * p.tiles), (unsigned)((slots + 7) / 8)), dim3(64 * pkv::kWaves), 0,
-                           ctx->stream, c, a);
+        const dim3 grid(8, (unsigned)(kv->n_kv * p.tiles), (unsigned)((slots + 7) / 8));
+        hipLaunchKernelGGL((pkv_attend_kernel<decltype(hd)::value, decltype(elem)::value>), grid,
+                           dim3(64 * pkv::kWaves), 0, ctx->stream, c, a);
         if (join)
             hipLaunchKernelGGL((pkv_join_kernel<decltype(hd)::value>), dim3((unsigned)a.n_head, (unsigned)rows),
                                dim3(64 * kJoinWaves), 0, ctx->stream, c, a);
@@ -1155,7 +1155,8 @@ int64_t llmq_pkv_work_bytes(const llmq_pkv *kv, int64_t rows, int n_head) {
 int llmq_pkv_attend(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q, int64_t ldq,
                     int64_t rows, int n_head, const int32_t *len, const int32_t *table, int64_t width, float scale,
                     float cap, const float *slopes, void *work, int64_t work_bytes) {
-    Attend a{out, ldo, q, nullptr, nullptr, ldq, len, n_head, scale, cap, slopes, 0, 0, 0, 0, nullptr, nullptr, nullptr};
+    const Attend a{out, ldo, q, nullptr, nullptr, ldq, len, n_head, scale, cap, slopes, 0, 0, 0, 0, nullptr, nullptr,
+                   nullptr};
     return attend("pkv_attend", ctx, kv, layer, a, rows, table, width, work, work_bytes);
 }
 
@@ -1163,7 +1164,7 @@ int llmq_pkv_step(llmq_ctx *ctx, llmq_pkv *kv, int layer, float *out, int64_t ld
                   const float *v, int64_t ld, int64_t rows, int n_head, const int32_t *pos, const int32_t *table,
                   int64_t width, float scale, float cap, const float *slopes, void *work, int64_t work_bytes) {
     LLMQ_REQUIRE((k && v) || rows == 0, "pkv_step: null argument");
-    Attend a{out, ldo, q, k, v, ld, pos, n_head, scale, cap, slopes, 0, 0, 0, 0, nullptr, nullptr, nullptr};
+    const Attend a{out, ldo, q, k, v, ld, pos, n_head, scale, cap, slopes, 0, 0, 0, 0, nullptr, nullptr, nullptr};
     return attend("pkv_step", ctx, kv, layer, a, rows, table, width, work, work_bytes);
 }
 
