@@ -47,7 +47,7 @@ PKV_HD int64_t clamp_len(int64_t len, int64_t width, int page) {
 // second launch would have joined their parts.
 //
 // kWorkgroups: 2.7 times those that run at once.  4 rows of float16, 342 MB:
-// 1536 64.9 us, 2048 62.2, 3072 65; 64 rows of int8, 1082 MB: 199, 201, 204.
+// 1536 64.9 us, 2048 62.2, 2560 62.1; 64 rows of int8, 1082 MB: 199, 201, 202.
 // kPlanRows: 300 rows of up to 16384 positions and one head, each its own
 // workgroup 255 us, cut 139; 600 rows 203 and 151.
 constexpr int kWaves = 4;         // of a workgroup, each taking every kWaves-th block
