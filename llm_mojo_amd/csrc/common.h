@@ -98,14 +98,14 @@ int llmq_set_error(int code, const char *fmt, ...);
         if (rc_ != LLMQ_OK) return rc_; \
     } while (0)
 
-// The context's device is the current one while this lives.
+// A device (the context's) is the current one while this lives.
 struct DeviceGuard {
     int before = -1;
-    explicit DeviceGuard(const llmq_ctx *ctx) {
+    explicit DeviceGuard(int device) {
         int now = -1;
-        if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess)
-            before = now;
+        if (hipGetDevice(&now) == hipSuccess && now != device && hipSetDevice(device) == hipSuccess) before = now;
     }
+    explicit DeviceGuard(const llmq_ctx *ctx) : DeviceGuard(ctx->device) {}
     ~DeviceGuard() {
         if (before >= 0) (void)hipSetDevice(before);
     }

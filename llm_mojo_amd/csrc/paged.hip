@@ -13,8 +13,7 @@
 #include "paged_plan.h"
 
 struct llmq_pkv {
-    llmq_ctx *ctx = nullptr;
-    int type = 0, n_layer = 0, page = 0, n_kv = 0, hd = 0;
+    int device = 0, type = 0, n_layer = 0, page = 0, n_kv = 0, hd = 0;
     int64_t n_pages = 0;
     uint8_t *k = nullptr, *v = nullptr;
     float *ks = nullptr, *vs = nullptr;  // int8 only
@@ -969,8 +968,8 @@ int dispatch(const llmq_pkv *kv, F &&f) {
 int check_cache(const char *name, const llmq_ctx *ctx, const llmq_pkv *kv, int layer, const void *table,
                 int64_t width, int64_t rows) {
     LLMQ_REQUIRE(ctx && kv && (table || rows == 0), "%s: null argument", name);
-    LLMQ_REQUIRE(kv->ctx->device == ctx->device, "%s: the cache is on device %d, the context on %d", name,
-                 kv->ctx->device, ctx->device);
+    LLMQ_REQUIRE(kv->device == ctx->device, "%s: the cache is on device %d, the context on %d", name,
+                 kv->device, ctx->device);
     LLMQ_REQUIRE(layer >= 0 && layer < kv->n_layer, "%s: layer %d of %d", name, layer, kv->n_layer);
     LLMQ_REQUIRE(width >= 1 && width <= INT32_MAX / kv->page, "%s: a table row of %lld pages", name, (long long)width);
     return LLMQ_OK;
@@ -1068,7 +1067,7 @@ int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int p
     LLMQ_REQUIRE(total < 1e15, "pkv_create: %g elements", total);
     llmq_pkv *kv = new (std::nothrow) llmq_pkv();
     if (!kv) return llmq_set_error(LLMQ_ENOMEM, "pkv_create: out of host memory");
-    kv->ctx = ctx;
+    kv->device = ctx->device;
     kv->type = type;
     kv->n_layer = n_layer;
     kv->n_pages = n_pages;
@@ -1099,9 +1098,8 @@ int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int p
 
 int llmq_pkv_free(llmq_pkv *kv) {
     if (!kv) return LLMQ_OK;
-    DeviceGuard guard(kv->ctx);
-    hipStreamSynchronize(kv->ctx->stream);
-    hipFree(kv->k);
+    DeviceGuard guard(kv->device);
+    hipFree(kv->k);  // (waits for the device; the context may be gone)
     hipFree(kv->v);
     hipFree(kv->ks);
     hipFree(kv->vs);

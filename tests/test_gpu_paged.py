@@ -586,6 +586,27 @@ def test_streams(gpu):
     assert all(np.array_equal(o, base) for o in outs)
 
 
+def test_cache_outlives_its_context(gpu):
+    torch, lm, ctx = gpu
+    other = lm.Context(0)
+    c = lm.PagedKV(other, 1, 4, 64, 2, 64)
+    other.close()
+    assert c.nbytes() == 2 * 4 * 2 * 64 * (64 + 4)
+    z = lambda *s, **k: torch.zeros(*s, device="cuda", **k)  # noqa: E731
+    i = z(1, dtype=torch.int32)
+    with pytest.raises(lm.LlmqError):  # no context, no call
+        c.store(0, z(1, 2, 64), z(1, 2, 64), i, i, i[None])
+    c.ctx = ctx
+    c.store(0, z(1, 2, 64) + 3, z(1, 2, 64), i, i, i[None])
+    k, v = z(1, 2, 64), z(1, 2, 64)
+    c.fetch(0, k, v, i, i, i[None])
+    assert np.allclose(k.cpu().numpy(), 3)
+    c.free()
+    with pytest.raises(lm.LlmqError):
+        c.fetch(0, k, v, i, i, i[None])
+    c.free()
+
+
 def test_refusals(gpu):
     torch, lm, ctx = gpu
     for args in ((0, 4, 64, 2, 64), (1, 0, 64, 2, 64), (1, 4, 32, 2, 64), (1, 4, 96, 2, 64), (1, 4, 8192, 2, 64),
