@@ -21,7 +21,6 @@ import math
 import torch
 
 own = False
-opened = []
 
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -175,21 +174,13 @@ def logit_inputs(case, g):
     return s
 
 
-def library():
-    """The package, and the one context and stream that a program has: every state's calls go there."""
-    if not opened:
-        import llm_mojo_amd as lm
-
-        stream = torch.cuda.Stream()
-        opened.append((lm, lm.Context(0, stream), stream))
-    return opened[0]
-
-
 def prepare(case, seed):
     g = generator(seed)
     s = {"case": case}
     if own:
-        s["lm"], s["ctx"], s["stream"] = library()
+        import llm_mojo_amd as lm
+
+        s["lm"], s["ctx"] = lm, lm.Context(0, torch.cuda.current_stream())
     if case["kind"] in ("step", "store"):
         kv, hd, page = case["kv"], case["hd"], case["page"]
         s["length"], s["table"], n_pages = paged(case, seed, g)
@@ -215,9 +206,7 @@ def prepare(case, seed):
             s["all"] = torch.arange(n, dtype=torch.int32, device="cuda")
             s["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads) if case["bias"] else None
             if own:
-                s["stream"].wait_stream(torch.cuda.current_stream())
                 s["cache"].store(0, k, v, seq, pos, s["table"])
-                torch.cuda.current_stream().wait_stream(s["stream"])
                 s["work"] = torch.empty(s["cache"].work_bytes(n, heads), dtype=torch.uint8, device="cuda")
                 s["ko"], s["vo"] = torch.empty(n, kv, hd, device="cuda"), torch.empty(n, kv, hd, device="cuda")
             else:
@@ -239,9 +228,7 @@ def prepare(case, seed):
         s["resid"] = normal(g, t, n) if case["resid"] else None
         s["out"] = torch.zeros(t, n, device="cuda")
         if own:
-            s["stream"].wait_stream(torch.cuda.current_stream())
             s["w"] = s["lm"].HipMX4Matrix.from_f32(s["ctx"], w, reduce_rows=False)
-            torch.cuda.current_stream().wait_stream(s["stream"])
         else:
             s["w"] = pack(*mx4(w))
     else:
@@ -407,8 +394,7 @@ def run(s):
     if c["kind"] == "linear":
         if own:
             if c["resid"]:
-                with torch.cuda.stream(s["stream"]):
-                    s["out"].copy_(s["resid"])
+                s["out"].copy_(s["resid"])
             s["lm"].linear(s["ctx"], s["out"], s["x"], s["w"], s["b"], resid=c["resid"], gelu=c["gelu"])
             return s["out"]
         return plain_linear(s)
