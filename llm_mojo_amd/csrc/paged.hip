@@ -337,7 +337,7 @@ struct Attend {
     int rows, tiles, columns;  // columns 0: a workgroup a row
     uint32_t least;            // of the plan
     int2 *meta;   // [row]: first slot, segments
-    float2 *ml;   // [slot][head]: reference (log2), sum
+    float2 *ml;   // [slot][head]: reference, sum
     float *sums;  // [slot][head][hd]
 };
 
@@ -511,6 +511,9 @@ __device__ __forceinline__ int table_at(const int32_t *p) {
 //
 // The reference of a head's exponentials is moved (and the sums rescaled)
 // only when a score passes it by 4, which is rare after the first blocks.
+// Scores are compared and taken by their difference from it, which is exact
+// where it matters: the reference times log2 e would be off by whole units
+// from 2^24 on, and infinite above 2.3e38.
 // Each wave keeps its own and reads every fourth block; they are put
 // together through LDS.  A wave's next keys are on their way while it forms
 // the weights, its next values while it scores.
@@ -695,7 +698,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     v4f acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = kLowest, ref2 = kLowest, l = 0.0f;  // ref2 = ref log2 e, rounded once
+    float ref = kLowest, l = 0.0f;
     int ve = ELEM == 1 ? -100 : 0;                   // the weights' power of two
 
     // one block; LAST: the wave's last, which may hold the new token and the
@@ -811,11 +814,10 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
             vm = quarters_max(vm);
             nve = max(ve, (int)(__float_as_uint(vm) >> 23) - 127);
         }
-        if (__any(mx > ref + 4.0f || nve > ve)) {  // exponentials stay below 2^6
-            const float to = fmaxf(ref, mx), to2 = to * kLog2e;
-            const float f = ref == to ? 1.0f : exp2f(ref2 - to2), fl = ldexpf(f, ve - nve);
+        if (__any(mx - ref > 4.0f || nve > ve)) {  // exponentials stay below 2^6
+            const float to = fmaxf(ref, mx);
+            const float f = ref == to ? 1.0f : exp2f((ref - to) * kLog2e), fl = ldexpf(f, ve - nve);
             ref = to;
-            ref2 = ref == kLowest ? kLowest : to2;
             ve = nve;
             l *= f;
 #pragma unroll
@@ -829,7 +831,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         h8 wf;
 #pragma unroll
         for (int i = 0; i < NT * 4; i++) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sv[i], kLog2e, -ref2));
+            const float p = __builtin_amdgcn_exp2f((sv[i] - ref) * kLog2e);
             l += p;
             float y = ELEM == 1 ? p * (vs[i >> 2][i & 3] * unit) : p * unit;
             // rounded to 32 bits once, for both rows: the product straight to 16 bits would now and then be another
@@ -852,7 +854,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     if (b < b1) block(std::true_type{});
     // the waves' results
     l = quarters_sum(l);
-    if (lane < 8) wml[w][n] = make_float2(ref2, l);
+    if (lane < 8) wml[w][n] = make_float2(ref, l);
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -869,7 +871,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         for (int k = 0; k < pkv::kWaves; k++) R = fmaxf(R, wml[k][h].x);
 #pragma unroll
         for (int k = 0; k < pkv::kWaves; k++) {
-            const float f = exp2f(wml[k][h].x - R);
+            const float f = exp2f((wml[k][h].x - R) * kLog2e);
             L = fmaf(wml[k][h].y, f, L);
             o = fmaf(wsum[k][h][d], f, o);
         }
@@ -924,14 +926,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Atte
         float to = R;
 #pragma unroll
         for (int k = 0; k < kAtOnce; k++) to = fmaxf(to, x[k].x);
-        const float f = exp2f(R - to);
+        const float f = exp2f((R - to) * kLog2e);
         R = to;
         L *= f;
 #pragma unroll
         for (int d = 0; d < HD / 64; d++) o[d] *= f;
 #pragma unroll
         for (int k = 0; k < kAtOnce; k++) {
-            const float g = exp2f(x[k].x - R);
+            const float g = exp2f((x[k].x - R) * kLog2e);
             L = fmaf(x[k].y, g, L);
 #pragma unroll
             for (int d = 0; d < HD / 64; d++) o[d] = fmaf(s[k][d], g, o[d]);
@@ -948,7 +950,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void pkv_join_kernel(Layer c, Atte
         for (int k = 0; k < kJoinWaves; k++) to = fmaxf(to, wl[k].x);
 #pragma unroll
         for (int k = 0; k < kJoinWaves; k++) {
-            const float g = exp2f(wl[k].x - to);
+            const float g = exp2f((wl[k].x - to) * kLog2e);
             all = fmaf(wl[k].y, g, all);
             s = fmaf(ws[k][d], g, s);
         }
