@@ -506,11 +506,17 @@ __device__ __forceinline__ int table_at(const int32_t *p) {
 // the weights are already where the second product wants its rows: row n
 // holds head n's weights as float16, row n ^ 8 what is left times 2^11, and
 // the slots of paged_plan.h give the values in the same order, so nothing is
-// moved between lanes.  For int8 a weight is p times the value's scale over a
-// power of two near the largest scale so far.
+// moved between lanes.  For int8 a weight is p times the value's scale.
+//
+// Weights are put near float16's upper end by a power of two: for float16 a
+// constant, for int8 one a head that follows its largest weight so far (not
+// its largest scale: a large value behind a low score would take the bits of
+// all others).  So a weight is held to 2^-22 of itself, and to 2^-48 of its
+// head's largest.
 //
 // The reference of a head's exponentials is moved (and the sums rescaled)
-// only when a score passes it by 4, which is rare after the first blocks.
+// only when a score passes it by 1, which is rare after the first blocks, as
+// is a weight that outgrows its power of two by 4.
 // Scores are compared and taken by their difference from it, which is exact
 // where it matters: the reference times log2 e would be off by whole units
 // from 2^24 on, and infinite above 2.3e38.
@@ -699,7 +705,9 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
 #pragma unroll
     for (int d = 0; d < ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float ref = kLowest, l = 0.0f;
-    int ve = ELEM == 1 ? -100 : 0;                   // the weights' power of two
+    // the weights' power of two: p is at most e (e 2^14 < 65504), a weight for int8 below 2^(ve + 2)
+    constexpr int kTop = ELEM == 1 ? 13 : 14, kLeast = -100;
+    int ve = ELEM == 1 ? kLeast : 0;
 
     // one block; LAST: the wave's last, which may hold the new token and the
     // row's end (the others are whole, or in a page that is none)
@@ -806,34 +814,41 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
 #pragma unroll
         for (int i = 1; i < NT * 4; i++) mx = fmaxf(mx, sv[i]);
         mx = quarters_max(mx);
-        int nve = ve;
-        if constexpr (ELEM == 1) {
-            float vm = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NT * 4; i++) vm = fmaxf(vm, vs[i >> 2][i & 3]);
-            vm = quarters_max(vm);
-            nve = max(ve, (int)(__float_as_uint(vm) >> 23) - 127);
-        }
-        if (__any(mx - ref > 4.0f || nve > ve)) {  // exponentials stay below 2^6
+        const bool moves = __any(mx - ref > 1.0f);
+        float down = 0.0f;  // log2 of what the sums so far are multiplied by
+        if (moves) {
             const float to = fmaxf(ref, mx);
-            const float f = ref == to ? 1.0f : exp2f((ref - to) * kLog2e), fl = ldexpf(f, ve - nve);
+            down = ref == to ? 0.0f : (ref - to) * kLog2e;
             ref = to;
-            ve = nve;
-            l *= f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float y = __shfl(fl, 4 * q + i);  // of row 4 q + i
-#pragma unroll
-                for (int d = 0; d < ND; d++) acc[d][i] *= y;
-            }
+            l *= exp2f(down);
         }
-        const float unit = ldexpf(1.0f, 8 - ve);
-        h8 wf;
+        float wm = 0.0f;
 #pragma unroll
         for (int i = 0; i < NT * 4; i++) {
             const float p = __builtin_amdgcn_exp2f((sv[i] - ref) * kLog2e);
             l += p;
-            float y = ELEM == 1 ? p * (vs[i >> 2][i & 3] * unit) : p * unit;
+            sv[i] = ELEM == 1 ? p * vs[i >> 2][i & 3] : p;
+            if constexpr (ELEM == 1) wm = fmaxf(wm, sv[i]);
+        }
+        int e = 0;
+        if constexpr (ELEM == 1) e = (int)(__float_as_uint(quarters_max(wm)) >> 23) - 127;
+        if (moves || (ELEM == 1 && __any(e > ve + 1))) {
+            int to = ve;
+            if constexpr (ELEM == 1) to = max(max(ve + (int)floorf(fmaxf(down, -400.0f)), e), kLeast);
+            const float f = ldexpf(exp2f(down), ve - to);
+            ve = to;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float y = __shfl(f, 4 * q + i);  // of row 4 q + i
+#pragma unroll
+                for (int d = 0; d < ND; d++) acc[d][i] *= y;
+            }
+        }
+        const float unit = ldexpf(1.0f, kTop - ve);
+        h8 wf;
+#pragma unroll
+        for (int i = 0; i < NT * 4; i++) {
+            float y = sv[i] * unit;
             // rounded to 32 bits once, for both rows: the product straight to 16 bits would now and then be another
             // float16 than the one below, and the rows no longer add up
             asm volatile("" : "+v"(y));
@@ -856,12 +871,14 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     l = quarters_sum(l);
     if (lane < 8) wml[w][n] = make_float2(ref, l);
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+    for (int i = 0; i < 4; i++) {
+        const int e = ELEM == 1 ? __shfl(ve, 4 * q + i) : 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int d = 0; d < ND; d++) {
             const float y = acc[d][i], z = __shfl_xor(y, 32);  // rows 4 q + i and 4 q + i + 8
-            if (q < 2) wsum[w][4 * q + i][16 * d + n] = ldexpf(fmaf(z, 0x1p-11f, y), ve - 8);
+            if (q < 2) wsum[w][4 * q + i][16 * d + n] = ldexpf(fmaf(z, 0x1p-11f, y), e - kTop);
         }
+    }
     __syncthreads();
     if (tid == 0 && blockIdx.y == 0 && a.columns && b0 == 0) a.meta[r] = make_int2(slot, count);
     for (int i = tid; i < hn * HD; i += 64 * pkv::kWaves) {

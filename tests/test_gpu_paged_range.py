@@ -1,11 +1,11 @@
 """The paged cache's attention at the ends of its types' ranges: scores far
-from zero, whose differences float32 still holds."""
+from zero, whose differences float32 still holds; values of very unlike sizes."""
 import math
 
 import numpy as np
 import pytest
 
-from tests.test_gpu_paged import KINDS, Case, dev, held
+from tests.test_gpu_paged import KINDS, Case, dev, held, want
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,48 @@ def test_scores_far_from_zero(gpu, kind, exponent, sign, lens, width):
             p /= p.sum()
             bar = (2.0 ** -17 + 2.0 ** -20 + (n / 16 + 64) * 2.0 ** -24) * (p @ np.abs(v[at])) + 1e-37
             assert np.all(np.abs(got[r, h] - p @ v[at]) <= bar), (r, h)
+
+
+@pytest.mark.parametrize("where", ["one", "first", "last", "spread"])
+@pytest.mark.parametrize("r", [20, 28, 36, 50, 80])
+def test_large_values_behind_low_scores(gpu, r, where):
+    """Positions whose values are 2^r times the others' and whose scores lie
+    100 below them take nothing from the others, for half of the heads; for
+    the other half they are all there is.  The bar is the other tests': a
+    share of sum p |v|."""
+    for lens, width in (([260, 40], None), ([2500, 33, 700], 50)):
+        c = Case(gpu, "int8", 64, 2, lens, width=width, seed=r)
+        n = np.array(lens)[c.seq]
+        large = {"one": c.pos == n * 2 // 3, "first": c.pos < n // 2, "last": c.pos >= n // 2, "spread": c.pos % 5 == 1}[where]
+        w = c.rng.normal(0, 1, 64).astype(np.float32)
+        c.k *= np.float32(0.3)
+        c.k[large] = (-800 / (w @ w)) * w
+        c.v *= np.where(large, np.float32(2.0 ** (r / 2)), np.float32(2.0 ** (-r / 2)))[:, None, None]
+        put(c)
+        q = (c.rng.normal(0, 0.01, (len(lens), 8, 64)) + w * np.array([1, -1] * 4)[:, None]).astype(np.float32)
+        _, got = c.attend(8, q=q)
+        k, v = held("int8", c.k), held("int8", c.v)
+        for i in range(len(lens)):
+            at = c.rows(i)
+            o, bar = want(q[i], k[at], v[at], 0.125, 0.0, None)
+            assert np.all(np.abs(got[i] - o) <= bar), (lens, i)
+
+
+def test_values_outgrown_as_scores_rise(gpu):
+    """Scores that rise by 3 a block while the values' scale falls by 2^5 a
+    block: the largest weight is a new position's, then an old one's."""
+    for step, fall in ((3.0, 5.0), (3.0, 4.0), (6.0, 5.0), (-3.0, -5.0), (-6.0, -5.0)):
+        c = Case(gpu, "int8", 64, 1, [640, 900], width=40)
+        block = c.pos // 32
+        c.k *= np.float32(0.05)
+        c.k[:, 0, 0] = block * step
+        c.v *= (2.0 ** (-fall * (block - 14))).astype(np.float32)[:, None, None]
+        put(c)
+        q = c.rng.normal(0, 1, (2, 3, 64)).astype(np.float32)
+        q[:, :, 0] = 8
+        _, got = c.attend(3, q=q)
+        k, v = held("int8", c.k), held("int8", c.v)
+        for i in range(2):
+            at = c.rows(i)
+            o, bar = want(q[i], k[at], v[at], 0.125, 0.0, None)
+            assert np.all(np.abs(got[i] - o) <= bar), (step, fall, i)
