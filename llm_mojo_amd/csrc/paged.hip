@@ -501,8 +501,10 @@ __device__ __forceinline__ int table_at(const int32_t *p) {
 //
 // Scores: K (16 positions x 32 dimensions) times the queries as 16 columns,
 // columns 0-7 their float16 roundings and 8-15 what those leave times 2^11
-// (22 bits in all; the keys are exact), so columns n and n ^ 8 add up to a
-// score, in lane n for positions 4 (lane / 16) + 0..3 of the tile.  Values:
+// (the keys are exact), so columns n and n ^ 8 add up to a score, in lane n
+// for positions 4 (lane / 16) + 0..3 of the tile.  A head's queries are put by
+// a power of two to where the largest is just below float16's end, 2^15: each
+// is held to 2^-23 of itself, and to 2^-50 of the largest.  Values:
 // the weights are already where the second product wants its rows: row n
 // holds head n's weights as float16, row n ^ 8 what is left times 2^11, and
 // the slots of paged_plan.h give the values in the same order, so nothing is
@@ -659,7 +661,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
                 m = fmaxf(m, fabsf(x[f][i]));
             }
         m = quarters_max(m);
-        const int e = m > 0.0f ? (int)(__float_as_uint(m) >> 23) - 127 : 0;
+        const int e = max((int)(__float_as_uint(m) >> 23) - (127 + 14), -112);  // (mul stays a normal float)
         mul = ldexpf(a.scale, e);
 #pragma unroll
         for (int f = 0; f < NF; f++)
@@ -771,9 +773,8 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float y = s[t][i] * own + llmq_dppf<0x128>(s[t][i]) * oth;  // row_ror:8
-                if constexpr (ELEM == 1) y *= ks[t][i];
-                sv[4 * t + i] = y * mul;
+                const float y = s[t][i] * own + llmq_dppf<0x128>(s[t][i]) * oth;  // row_ror:8
+                sv[4 * t + i] = y * (ELEM == 1 ? ks[t][i] * mul : mul);
             }
         if constexpr (!LAST) load_k();
         if (a.cap > 0.0f)

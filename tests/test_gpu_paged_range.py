@@ -1,5 +1,5 @@
 """The paged cache's attention at the ends of its types' ranges: scores far
-from zero, whose differences float32 still holds; values of very unlike sizes."""
+from zero, whose differences float32 still holds; queries and values of very unlike sizes."""
 import math
 
 import numpy as np
@@ -95,3 +95,37 @@ def test_values_outgrown_as_scores_rise(gpu):
             at = c.rows(i)
             o, bar = want(q[i], k[at], v[at], 0.125, 0.0, None)
             assert np.all(np.abs(got[i] - o) <= bar), (step, fall, i)
+
+
+@pytest.mark.parametrize("down", [16, 20, 24, 28])
+@pytest.mark.parametrize("kind", KINDS)
+def test_small_queries_beside_a_large_one(gpu, kind, down):
+    """A head's largest query meets keys of zero: the scores come from queries
+    2^-down of it, held as well as any other."""
+    c = Case(gpu, kind, 64, 2, [300, 5, 64])
+    c.k[:, :, 7] = 0
+    put(c)
+    q = c.rng.normal(0, 1.5 * 2.0 ** -down, (3, 4, 64)).astype(np.float32)
+    q[:, :, 7] = 3.0
+    scale = 2.0 ** down / 8
+    _, got = c.attend(4, scale=scale, q=q)
+    k, v = held(kind, c.k), held(kind, c.v)
+    for r in range(3):
+        at = c.rows(r)
+        o, bar = want(q[r], k[at], v[at], scale, 0.0, None)
+        assert np.all(np.abs(got[r] - o) <= bar), r
+
+
+def test_large_keys_and_small_queries(gpu):
+    """int8 keys near float32's end and queries as small: neither factor of a score may overflow before both are in."""
+    for up, scale in ((-100, 0.125), (100, 0.125), (117, 0.125), (117, 0.1), (112, 0.003)):
+        c = Case(gpu, "int8", 64, 1, [200, 33])
+        c.k *= np.float32(2.0 ** up)
+        put(c)
+        q = (c.rng.normal(0, 1.5, (2, 4, 64)) * 2.0 ** -up).astype(np.float32)
+        _, got = c.attend(4, q=q, scale=scale)
+        k, v = held("int8", c.k), held("int8", c.v)
+        for r in range(2):
+            at = c.rows(r)
+            o, bar = want(q[r], k[at], v[at], scale, 0.0, None)
+            assert np.all(np.abs(got[r] - o) <= bar), (up, r)
