@@ -65,7 +65,7 @@ __device__ __forceinline__ int row_code(float x, float inv) {
 
 __device__ __forceinline__ uint16_t half_bits(float x) {
     // nearest even; finite values past the range become its ends
-    const float lim = fabsf(x) <= 3.0e38f ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
+    const float lim = fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
     return __half_as_ushort(__float2half_rn(lim));
 }
 

@@ -129,3 +129,34 @@ def test_large_keys_and_small_queries(gpu):
             at = c.rows(r)
             o, bar = want(q[r], k[at], v[at], scale, 0.0, None)
             assert np.all(np.abs(got[r] - o) <= bar), (up, r)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_largest_floats(gpu, kind):
+    """Finite rows up to float32's largest, by store and by a step: float16
+    keeps its own largest for them, int8 their codes; infinities stay apart."""
+    torch, lm, ctx = gpu
+    big = [65504.0, 65519.0, 65520.0, 3e38, 3.1e38, 3.4028234663852886e38]
+    x = np.ones((2 * len(big), 1, 64), np.float32)
+    x[:, 0, 5] = np.array(big + [-b for b in big], np.float32)
+    n = len(x)
+    c = Case(gpu, kind, 64, 1, [n + 1])
+    c.cache.store(0, dev(torch, x), dev(torch, x), dev(torch, np.zeros(n, np.int32)), dev(torch, np.arange(n, dtype=np.int32)),
+                  c.table)
+    k, v = (torch.zeros(n, 1, 64, device="cuda") for _ in range(2))
+    c.cache.fetch(0, k, v, dev(torch, np.zeros(n, np.int32)), dev(torch, np.arange(n, dtype=np.int32)), c.table)
+    assert np.array_equal(k.cpu().numpy(), held(kind, x)) and np.array_equal(v.cpu().numpy(), held(kind, x))
+    w, _ = c.work(1, 1)
+    pos, zero = (dev(torch, np.array([i], np.int32)) for i in (n, 0))
+    for row in x:
+        r = dev(torch, row[None])
+        out = torch.zeros(1, 1, 64, device="cuda")
+        c.cache.step(0, out, torch.zeros(1, 1, 64, device="cuda"), r, r, pos, c.table, w)
+        c.cache.fetch(0, k[:1], v[:1], zero, pos, c.table)
+        assert np.array_equal(k[:1].cpu().numpy(), held(kind, row[None])) and torch.equal(k[:1], v[:1])
+        assert bool(out.isfinite().all()) or kind == "int8"  # (a sum of 13 values near float32's end)
+    if kind == "f16":
+        inf = torch.full((1, 1, 64), float("inf"), device="cuda")
+        c.cache.store(0, inf, -inf, zero, pos, c.table)
+        c.cache.fetch(0, k[:1], v[:1], zero, pos, c.table)
+        assert torch.equal(k[:1], inf) and torch.equal(v[:1], -inf)
