@@ -221,7 +221,7 @@ static int mat_alloc_quant(llmq_ctx *ctx, int bits, int group, int sym, int a16,
     RC(quant_shape_ok(bits, group, a16, n, k));
     const int64_t g = group == 0 ? k : group;
     llmq_mat *m = new llmq_mat();
-    m->ctx = ctx;
+    m->device = ctx->device;
     m->kind = MAT_QUANT;
     m->bits = bits;
     m->group_param = group;
@@ -287,8 +287,8 @@ int llmq_mat_from_f32(llmq_ctx *ctx, int bits, int group, int sym, int a16, cons
 
 int llmq_mat_free(llmq_mat *m) {
     if (!m) return LLMQ_OK;
-    if (m->ctx) hipStreamSynchronize(m->ctx->stream);
-    hipFree(m->codes);
+    DeviceGuard guard(m->device);
+    hipFree(m->codes);  // (waits for the device; the context may be gone)
     hipFree(m->scales);
     hipFree(m->zps);
     hipFree(m->blocks);
@@ -482,7 +482,7 @@ int llmq_mat_from_gguf(llmq_ctx *ctx, int ggml_type, const void *blocks, int64_t
         return llmq_set_error(LLMQ_EUNSUPPORTED, "from_gguf: ggml type %d is not a supported block format",
                               ggml_type);
     llmq_mat *m = new llmq_mat();
-    m->ctx = ctx;
+    m->device = ctx->device;
     int rc = gguf_upload(ctx, m, ggml_type, static_cast<const uint8_t *>(blocks), rows, cols);
     if (rc != LLMQ_OK) {
         llmq_mat_free(m);

@@ -54,7 +54,7 @@ bool ctx_capturing(const llmq_ctx *ctx);
 enum { MAT_QUANT = 0, MAT_GGUF = 1, MAT_MX4 = 2 };
 
 struct llmq_mat {
-    llmq_ctx *ctx = nullptr;
+    int device = -1;  // its memory's
     int kind = MAT_QUANT;
     // QuantMatrix
     int bits = 0, group_param = 0, sym = 0, a16 = 0;

@@ -643,7 +643,7 @@ int check_shape(const char *name, int64_t rows, int64_t cols) {
 int mx4_alloc(llmq_ctx *ctx, int64_t n, int64_t k, llmq_mat **out) {
     llmq_mat *m = new (std::nothrow) llmq_mat();
     if (!m) return llmq_set_error(LLMQ_ENOMEM, "from_f32_mx4: out of host memory");
-    m->ctx = ctx;
+    m->device = ctx->device;
     m->kind = MAT_MX4;
     m->bits = 4;
     m->n = n;
