@@ -640,6 +640,13 @@ int check_shape(const char *name, int64_t rows, int64_t cols) {
     return LLMQ_OK;
 }
 
+// A matrix is used on its own GPU, whose memory it is in.
+int check_device(const char *name, const llmq_ctx *ctx, const llmq_mat *m) {
+    LLMQ_REQUIRE(m->device == ctx->device, "%s: the matrix is on device %d, the context on %d", name, m->device,
+                 ctx->device);
+    return LLMQ_OK;
+}
+
 int mx4_alloc(llmq_ctx *ctx, int64_t n, int64_t k, llmq_mat **out) {
     llmq_mat *m = new (std::nothrow) llmq_mat();
     if (!m) return llmq_set_error(LLMQ_ENOMEM, "from_f32_mx4: out of host memory");
@@ -802,6 +809,7 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
                       int flags, void *rec, int64_t rec_cap) {
     RC(check_epilogue("linear", out, bias, T, flags));
     LLMQ_REQUIRE(T >= 0 && T <= INT32_MAX && (x || T == 0), "linear: %lld microscaled tokens", (long long)T);
+    RC(check_device("linear", ctx, w));
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
     // one token's row fits LDS beside the sums
@@ -832,6 +840,7 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
 }
 
 int mx4_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *dst) {
+    RC(check_device("dequant_row", ctx, m));
     DeviceGuard guard(ctx);
     try {
         const int64_t nb = m->k / 32, tile = row >> 4, r = row & 15;
@@ -956,6 +965,7 @@ int llmq_mat_restore_mx4(llmq_ctx *ctx, int64_t rows, int64_t cols, const uint8_
 
 int llmq_mat_export_mx4(llmq_ctx *ctx, const llmq_mat *m, uint8_t *codes, uint8_t *scales) {
     LLMQ_REQUIRE(ctx && m && m->kind == MAT_MX4, "export_mx4: not a microscaled matrix");
+    RC(check_device("export_mx4", ctx, m));
     DeviceGuard guard(ctx);
     try {
         std::vector<uint8_t> c((size_t)(m->ntiles * m->NG) * 4096), s((size_t)(m->ntiles * m->NG) * 256);
@@ -982,6 +992,7 @@ int llmq_mx4_linear(llmq_ctx *ctx, float *out, const uint8_t *codes, const uint8
     LLMQ_REQUIRE(w->k == IN && w->n == OUT, "mx4_linear: matrix is %lldx%lld, call says IN=%lld OUT=%lld",
                  (long long)w->n, (long long)w->k, (long long)IN, (long long)OUT);
     RC(check_codes("mx4_linear", ctx, out, codes, scales, T, IN));
+    RC(check_device("mx4_linear", ctx, w));
     RC(check_epilogue("mx4_linear", out, bias, T, flags));
     if (T == 0) return LLMQ_OK;
     DeviceGuard guard(ctx);
