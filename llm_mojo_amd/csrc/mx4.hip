@@ -647,6 +647,12 @@ int check_device(const char *name, const llmq_ctx *ctx, const llmq_mat *m) {
     return LLMQ_OK;
 }
 
+// Calls that allocate, or copy to or from host memory, cannot be part of a graph.
+int check_no_capture(const char *name, const llmq_ctx *ctx) {
+    LLMQ_REQUIRE(!ctx_capturing(ctx), "%s: not under graph capture", name);
+    return LLMQ_OK;
+}
+
 int mx4_alloc(llmq_ctx *ctx, int64_t n, int64_t k, llmq_mat **out) {
     llmq_mat *m = new (std::nothrow) llmq_mat();
     if (!m) return llmq_set_error(LLMQ_ENOMEM, "from_f32_mx4: out of host memory");
@@ -841,6 +847,7 @@ int launch_mx4_linear(llmq_ctx *ctx, const llmq_mat *w, const float *x, int64_t 
 
 int mx4_dequant_row(llmq_ctx *ctx, const llmq_mat *m, int64_t row, float *dst) {
     RC(check_device("dequant_row", ctx, m));
+    RC(check_no_capture("dequant_row", ctx));
     DeviceGuard guard(ctx);
     try {
         const int64_t nb = m->k / 32, tile = row >> 4, r = row & 15;
@@ -897,6 +904,7 @@ int llmq_mat_from_f32_mx4_device(llmq_ctx *ctx, const float *src, int64_t rows, 
     RC(check_shape("from_f32_mx4", n, k));
     const int64_t nb = k / 32, grid = (n * nb + 255) / 256;
     LLMQ_REQUIRE(grid <= INT32_MAX, "from_f32_mx4: %lld x %lld matrix", (long long)n, (long long)k);
+    RC(check_no_capture("from_f32_mx4", ctx));
     DeviceGuard guard(ctx);
     llmq_mat *m = nullptr;
     RC(mx4_alloc(ctx, n, k, &m));
@@ -915,6 +923,7 @@ int llmq_mat_from_f32_mx4(llmq_ctx *ctx, const float *src, int64_t rows, int64_t
                           llmq_mat **out) {
     LLMQ_REQUIRE(ctx && src && out, "from_f32_mx4: null argument");
     RC(check_shape("from_f32_mx4", reduce_rows ? cols : rows, reduce_rows ? rows : cols));
+    RC(check_no_capture("from_f32_mx4", ctx));
     DeviceGuard guard(ctx);
     float *d = nullptr;
     const size_t bytes = sizeof(float) * (size_t)rows * (size_t)cols;
@@ -925,9 +934,15 @@ int llmq_mat_from_f32_mx4(llmq_ctx *ctx, const float *src, int64_t rows, int64_t
     int rc = LLMQ_OK;
     if (hipMemcpyAsync(d, src, bytes, hipMemcpyHostToDevice, ctx->stream) != hipSuccess)
         rc = llmq_set_error(LLMQ_EHIP, "from_f32_mx4: copy to the device failed");
-    if (rc == LLMQ_OK) rc = llmq_mat_from_f32_mx4_device(ctx, d, rows, cols, reduce_rows, out);
-    hipStreamSynchronize(ctx->stream);
+    llmq_mat *m = nullptr;
+    if (rc == LLMQ_OK) rc = llmq_mat_from_f32_mx4_device(ctx, d, rows, cols, reduce_rows, &m);
+    const hipError_t e = hipStreamSynchronize(ctx->stream);
+    if (rc == LLMQ_OK && e != hipSuccess) {
+        llmq_mat_free(m);
+        rc = llmq_set_error(LLMQ_EHIP, "from_f32_mx4: %s", hipGetErrorString(e));
+    }
     hipFree(d);
+    if (rc == LLMQ_OK) *out = m;
     return rc;
 }
 
@@ -935,6 +950,7 @@ int llmq_mat_restore_mx4(llmq_ctx *ctx, int64_t rows, int64_t cols, const uint8_
                          llmq_mat **out) {
     LLMQ_REQUIRE(ctx && codes && scales && out, "restore_mx4: null argument");
     RC(check_shape("restore_mx4", rows, cols));
+    RC(check_no_capture("restore_mx4", ctx));
     DeviceGuard guard(ctx);
     llmq_mat *m = nullptr;
     RC(mx4_alloc(ctx, rows, cols, &m));
@@ -966,6 +982,7 @@ int llmq_mat_restore_mx4(llmq_ctx *ctx, int64_t rows, int64_t cols, const uint8_
 int llmq_mat_export_mx4(llmq_ctx *ctx, const llmq_mat *m, uint8_t *codes, uint8_t *scales) {
     LLMQ_REQUIRE(ctx && m && m->kind == MAT_MX4, "export_mx4: not a microscaled matrix");
     RC(check_device("export_mx4", ctx, m));
+    RC(check_no_capture("export_mx4", ctx));
     DeviceGuard guard(ctx);
     try {
         std::vector<uint8_t> c((size_t)(m->ntiles * m->NG) * 4096), s((size_t)(m->ntiles * m->NG) * 256);

@@ -1,4 +1,5 @@
-"""Microscaled matrices beside contexts that end before them, or are another GPU's."""
+"""Microscaled matrices beside contexts that end before them, are another GPU's, or are
+made while a stream is being captured."""
 import ctypes
 
 import numpy as np
@@ -61,3 +62,39 @@ def test_matrix_of_another_gpu(gpu):
     assert L.llmq_mat_dequant_row(far, m.h, 0, row.ctypes.data) == -1 and b"device" in L.llmq_last_error()
     assert L.llmq_mat_export_mx4(far, m.h, c.ctypes.data, s.ctypes.data) == -1 and b"device" in L.llmq_last_error()
     assert np.array_equal(m.dequant_row(0), np.ones(64, F))
+
+
+def test_matrices_are_not_made_under_capture(gpu):
+    """A matrix is made, and copied to the host, outside of graphs only: the
+    calls are refused before they touch the capture, which goes on."""
+    torch, lm, ctx = gpu
+    rng = np.random.default_rng(1)
+    w = rng.normal(0, 1, (16, 64)).astype(F)
+    wd = torch.from_numpy(w).cuda()
+    m = lm.HipMX4Matrix.from_f32(ctx, w, reduce_rows=False)
+    codes, scales = m.export()
+    x, out, want = torch.zeros(1, 64, device="cuda"), torch.zeros(1, 16, device="cuda"), torch.zeros(1, 16, device="cuda")
+    calls = [lambda: lm.HipMX4Matrix.from_f32(ctx, w, reduce_rows=False),
+             lambda: lm.HipMX4Matrix.from_f32(ctx, wd, reduce_rows=False),
+             lambda: lm.HipMX4Matrix.restore(ctx, codes, scales), m.export, lambda: m.dequant_row(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(side):
+            ctx.set_stream(side)
+            graph.capture_begin(capture_error_mode="relaxed")
+            for f in calls:
+                with pytest.raises(lm.LlmqError, match="capture"):
+                    f()
+            lm.linear(ctx, out, x, m)
+            graph.capture_end()
+    finally:
+        ctx.set_stream(torch.cuda.current_stream())
+    for i in range(3):
+        x.copy_(torch.from_numpy(rng.normal(0, 1, (1, 64)).astype(F)))
+        graph.replay()
+        lm.linear(ctx, want, x, m)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
