@@ -174,9 +174,11 @@ LLMQ_API int llmq_dot_row_i16(llmq_ctx *ctx, const llmq_mat *mat, int64_t row, i
  * may be NULL there).  Both operands of its products are microscaled:
  * llmq_linear, llmq_linear_noalloc and llmq_head quantize their rows of x as
  * above and then multiply (scratch of llmq_linear_noalloc: 17 / 32 bytes a
- * value, T rounded up to 16 and IN to 512); under graph capture llmq_linear refuses several
- * tokens (its workspace is the context's): quantize into memory of your own
- * and call llmq_mx4_linear. */
+ * value, T rounded up to 16 and IN to 512).  Under graph capture llmq_linear
+ * and llmq_head take one token of up to 122880 inputs and refuse the rest
+ * (their workspace is the context's): quantize into memory of your own and
+ * call llmq_mx4_linear.  Matrices are made, exported and read back outside of
+ * captures only, and used by contexts of their own GPU. */
 LLMQ_API int llmq_mat_from_f32_mx4(llmq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int reduce_rows,
                                    llmq_mat **out);
 LLMQ_API int llmq_mat_from_f32_mx4_device(llmq_ctx *ctx, const float *src, int64_t rows, int64_t cols,
@@ -333,10 +335,12 @@ LLMQ_API int llmq_ikv_export(llmq_ctx *ctx, const llmq_kv *kv, int8_t *k, int8_t
  *
  * Held per position and cached head: LLMQ_PKV_INT8 int8 codes with a float32
  * scale for the key and for the value, as QuantKV[8] (kvcache.mojo:248-385)
- * but for a scale's last bit: max|x| times the float 1 / 127 (a row with a
- * NaN or an infinity reads back as NaN, one below 2^-120 as zeros); LLMQ_PKV_F16 float16 values (nearest even, finite values past
- * 65504 saturate).  page: 64 to 4096 positions, a multiple of 64; head_dim
- * 64 or 128 (LLMQ_EUNSUPPORTED otherwise). */
+ * but for a scale's last bit: max|x| times the float 1 / 127, so a row's codes
+ * can differ from that cache's at ties (a row with a NaN or an infinity reads
+ * back as NaN, one below 2^-120 as zeros); LLMQ_PKV_F16 float16 values
+ * (nearest even, finite values past 65504 saturate).  page: 64 to 4096
+ * positions, a multiple of 64; head_dim 64 or 128 (LLMQ_EUNSUPPORTED
+ * otherwise). */
 typedef struct llmq_pkv llmq_pkv;
 enum { LLMQ_PKV_INT8 = 0, LLMQ_PKV_F16 = 1 };
 LLMQ_API int llmq_pkv_create(llmq_ctx *ctx, int type, int n_layer, int64_t n_pages, int page, int n_kv, int head_dim,
@@ -359,14 +363,22 @@ LLMQ_API int llmq_pkv_fetch(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float 
 /* Attention of one token a sequence: row r's n_head query heads (device
  * floats, rows ldq apart) over positions 0 .. len[r] - 1 of table row r,
  * query head h over cached head h / (n_head / n_kv):
- *   s_j = scale q . k_j;  s_j = cap tanh(s_j / cap) when cap > 0 (normal);
+ *   s_j = scale q . k_j;  s_j = cap tanh(s_j / cap) when cap > 0 (1.2e-38 to 3e38);
  *   s_j += slopes[h] (j - (len[r] - 1)) when slopes is given;
  *   out = sum_j softmax(s)_j v_j.
+ * Sums are in float32.  Their factors are held in two float16 parts each: a
+ * query to 2^-23 of itself but not below 2^-50 of its head's largest, a weight
+ * (exp(s_j - s_max), with LLMQ_PKV_INT8 times the value's scale) to 2^-22 of
+ * itself but not below 2^-48 of its head's largest; keys and values are exact
+ * as the cache holds them.
+ * A row's bits do not depend on what other rows hold, but its last ones may on
+ * their number and lengths, by which long rows are cut; the same call gives
+ * the same bits.
  * A length of 0 (or less) gives zeros; lengths past the table's row end with
  * it; positions in pages outside the cache are left out.  work: device
- * memory of llmq_pkv_work_bytes(kv, rows, n_head) bytes whose contents do
- * not matter, 16-byte aligned, not shared by calls that may overlap in time.  rows: at most
- * 65535. */
+ * memory of llmq_pkv_work_bytes(kv, rows, n_head) bytes (fewer rows may take
+ * more: above 1024 none is cut) whose contents do not matter, 16-byte aligned,
+ * not shared by calls that may overlap in time.  rows: at most 65535. */
 LLMQ_API int64_t llmq_pkv_work_bytes(const llmq_pkv *kv, int64_t rows, int n_head);
 LLMQ_API int llmq_pkv_attend(llmq_ctx *ctx, const llmq_pkv *kv, int layer, float *out, int64_t ldo, const float *q,
                              int64_t ldq, int64_t rows, int n_head, const int32_t *len, const int32_t *table,
@@ -415,8 +427,8 @@ typedef struct {
  * first token of the largest adjusted logit, as the reference's argmax; NaN is
  * never picked, and a row of nothing but -infinity and NaN gives -1.  work:
  * with pick, llmq_adjust_logits_work_bytes(rows, V) bytes of device memory
- * whose contents do not matter, 16-byte aligned, not shared by calls that may
- * overlap in time.  rows: at most 65535. */
+ * (fewer rows may take more) whose contents do not matter, 16-byte aligned,
+ * not shared by calls that may overlap in time.  rows: at most 65535. */
 LLMQ_API int64_t llmq_adjust_logits_work_bytes(int64_t rows, int64_t V);
 LLMQ_API int llmq_adjust_logits(llmq_ctx *ctx, float *out, int64_t ldo, const float *logits, int64_t ldl,
                                 int64_t rows, int64_t V, const llmq_logit_rules *rules, int64_t *pick, void *work,

@@ -149,10 +149,12 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const float *__restri
 
 // The same into a record: tokens in tiles of 16 laid out as a matrix's rows
 // are, so that a product's operand is 1 KB in one piece (rows of packed codes
-// 2 KB apart, at 4096 inputs, meet in few of L2's channels: 2048 x 4096 x
-// 11008 took 71 us from those and 61 from a record).  A workgroup 16 tokens and
-// a group of four steps, a wave a block of each step; tokens and blocks past
-// the end become zeros with scale 127.  2048 x 4096 takes 9-12 us after a
+// 2 KB apart, at 4096 inputs, meet in few of L2's channels, and the scales
+// that are gathered from them cost the product's kernel registers, 28 bytes of
+// scratch a lane with 96 tokens: 2048 x 4096 x 11008 takes 94 us from those and
+// 69 by way of a record, 2048 x 11008 x 4096 70 and 70).  A workgroup 16 tokens
+// and a group of four steps, a wave a block of each step; tokens and blocks
+// past the end become zeros with scale 127.  2048 x 4096 takes 9-12 us after a
 // product (7 alone; 38 MB).
 __global__ __launch_bounds__(256) void mx4_record_kernel(const float *__restrict__ x, int64_t T, int nb, int words,
                                                          uint32_t *__restrict__ codes, uint32_t *__restrict__ scales) {

@@ -62,7 +62,9 @@ class PagedKV:
     A table row (int32 [n_seq, width]) names a sequence's pages: position p is
     in page table[seq, p // page].  Positions, lengths and tables are device
     tensors, read when the kernels run.  kind "int8": int8 codes with a scale
-    a position and head, as QuantKV8; "f16": float16 values.
+    a position and head, as QuantKV8 but for the scale's last bit (max|x| times
+    the float 1 / 127, not over 127; codes can differ at ties); "f16": float16
+    values.
     """
 
     def __init__(self, ctx, n_layer, n_pages, page, n_kv, head_dim, kind="int8"):
@@ -80,7 +82,7 @@ class PagedKV:
         return lib().llmq_pkv_nbytes(self.h)
 
     def work_bytes(self, rows, n_head):
-        """Bytes of device memory that attend and step of `rows` rows take as `work`."""
+        """Bytes of device memory that attend and step of `rows` rows take as `work` (fewer rows may take more)."""
         return lib().llmq_pkv_work_bytes(self.h, rows, n_head)
 
     def _move(self, call, layer, k, v, seq, pos, table):
@@ -159,7 +161,7 @@ class PagedKV:
 
 
 def logits_work_bytes(rows, V):
-    """Bytes of device memory that adjust_logits takes as `work` for a pick."""
+    """Bytes of device memory that adjust_logits of `rows` rows takes as `work` for a pick (fewer rows may take more)."""
     return lib().llmq_adjust_logits_work_bytes(rows, V)
 
 
