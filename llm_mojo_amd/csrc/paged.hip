@@ -707,9 +707,11 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
 #pragma unroll
     for (int d = 0; d < ND; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float ref = kLowest, l = 0.0f;
-    // the weights' power of two: p is at most e (e 2^14 < 65504), a weight for int8 below 2^(ve + 2)
+    // the weights' power of two: p is at most e (e 2^14 < 65504), a weight for int8 below 2^(ve + 2); top is where it
+    // would be by the sums so far, which rising scores bring down by less than a power at a time
     constexpr int kTop = ELEM == 1 ? 13 : 14, kLeast = -100;
     int ve = ELEM == 1 ? kLeast : 0;
+    float top = kLeast;
 
     // one block; LAST: the wave's last, which may hold the new token and the
     // row's end (the others are whole, or in a page that is none)
@@ -835,7 +837,10 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         if constexpr (ELEM == 1) e = (int)(__float_as_uint(quarters_max(wm)) >> 23) - 127;
         if (moves || (ELEM == 1 && __any(e > ve + 1))) {
             int to = ve;
-            if constexpr (ELEM == 1) to = max(max(ve + (int)floorf(fmaxf(down, -400.0f)), e), kLeast);
+            if constexpr (ELEM == 1) {
+                top = fmaxf(fmaxf(top + fmaxf(down, -400.0f), (float)e), (float)kLeast);
+                to = (int)floorf(top);
+            }
             const float f = ldexpf(exp2f(down), ve - to);
             ve = to;
 #pragma unroll

@@ -160,3 +160,26 @@ def test_largest_floats(gpu, kind):
         c.cache.store(0, inf, -inf, zero, pos, c.table)
         c.cache.fetch(0, k[:1], v[:1], zero, pos, c.table)
         assert torch.equal(k[:1], inf) and torch.equal(v[:1], -inf)
+
+
+def test_old_values_beside_slowly_rising_scores(gpu):
+    """One head's scores rise by an eighth from each of a wave's blocks to the
+    next, the other's by more than 1, so that the reference moves each time;
+    the values of the first blocks are 2^200 times the others' and stay what
+    the first head's result is made of.  1025 rows, so that none is cut and a
+    wave has close to two hundred blocks."""
+    lens = [0] * 1025
+    lens[7] = 24000
+    c = Case(gpu, "int8", 64, 1, lens, page=256)
+    block = (c.pos // 32).astype(np.float32)
+    c.k[:] = 0
+    c.k[:, 0, 0] = c.k[:, 0, 1] = block
+    c.v *= np.where(block < 8, np.float32(2.0 ** 100), np.float32(2.0 ** -100))[:, None, None]
+    put(c)
+    q = np.zeros((1025, 2, 64), np.float32)
+    q[7, 0, 0], q[7, 1, 1] = 0.03125, 0.3
+    _, got = c.attend(2, scale=1.0, q=q)
+    at = c.rows(7)
+    o, bar = want(q[7], held("int8", c.k[at]), held("int8", c.v[at]), 1.0, 0.0, None)
+    assert np.all(np.abs(got[7] - o) <= bar)
+    assert not got[:7].any() and not got[8:].any()
