@@ -40,9 +40,10 @@ def _rows(t, heads, hd, dev, name):
     """Row stride of float32 [rows, heads, hd] (or [rows, heads * hd]) on GPU dev with whole rows in one piece."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 3:
-        ok = shape[1] == heads and shape[2] == hd and stride[2] == 1 and (heads == 1 or stride[1] == hd)
+        ok = (shape[1] == heads and shape[2] == hd
+              and (stride[2] == 1 and (heads == 1 or stride[1] == hd) or shape[0] == 0))
     else:
-        ok = len(shape) == 2 and shape[1] == heads * hd and stride[1] == 1
+        ok = len(shape) == 2 and shape[1] == heads * hd and (stride[1] == 1 or shape[0] == 0)
     if not ok or t.dtype is not torch.float32 or t.get_device() != dev:
         raise ValueError(f"{name}: a float32 tensor on GPU {dev} of rows of {heads} heads of {hd} in one piece, "
                          f"got {tuple(shape)} with strides {stride}")
@@ -186,7 +187,7 @@ def adjust_logits(ctx, out, logits, history=None, repetition=None, presence=None
     ld = []
     for t in (out, logits):
         stride = t.stride()
-        if t.shape != (rows, V) or t.dtype is not f32 or stride[1] != 1 or t.get_device() != dev:
+        if t.shape != (rows, V) or t.dtype is not f32 or (stride[1] != 1 and rows) or t.get_device() != dev:
             raise ValueError(f"logits and out: float32 [{rows}, {V}] on GPU {dev} with rows in one piece")
         ld.append(stride[0] if rows > 1 else max(stride[0], V))
     r = LogitRules()
@@ -209,7 +210,7 @@ def adjust_logits(ctx, out, logits, history=None, repetition=None, presence=None
     if mask is not None:
         words = mask.shape[1]
         stride = mask.stride()
-        if (mask.shape[0] != rows or 32 * words < V or stride[1] != 1 or mask.dtype is not i32
+        if (mask.shape[0] != rows or 32 * words < V or (stride[1] != 1 and rows) or mask.dtype is not i32
                 or mask.get_device() != dev):
             raise ValueError(f"mask: int32 words on GPU {dev}, {rows} rows of {V} bits")
         r.mask, r.mask_ld = mask.data_ptr(), stride[0] if rows > 1 else max(stride[0], words)
