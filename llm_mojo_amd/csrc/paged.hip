@@ -650,7 +650,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
     load_k();
     load_v();
     h8 qf[NF];
-    float mul;
+    float mul, big = 1.0f;  // a score's factors
     {
         float m = 0.0f;
 #pragma unroll
@@ -663,6 +663,10 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
         m = quarters_max(m);
         const int e = max((int)(__float_as_uint(m) >> 23) - (127 + 14), -112);  // (mul stays a normal float)
         mul = ldexpf(a.scale, e);
+        if (ELEM == 1 && e >= 0) {  // large queries: not with a key's scale, beside which it might overflow
+            big = mul;
+            mul = 1.0f;
+        }
 #pragma unroll
         for (int f = 0; f < NF; f++)
 #pragma unroll
@@ -672,7 +676,7 @@ __global__ __launch_bounds__(64 * pkv::kWaves, 3) void pkv_attend_kernel(Layer c
                 qf[f][i] = low ? (_Float16)((y - (float)hi) * 2048.0f) : hi;
             }
     }
-    const float own = low ? 0x1p-11f : 1.0f, oth = low ? 1.0f : 0x1p-11f;  // a score from the two columns
+    const float own = low ? 0x1p-11f * big : big, oth = low ? big : 0x1p-11f * big;  // a score from the two columns
     const float wg = low ? 2048.0f : 1.0f, wr = low ? -2048.0f : 0.0f;     // a weight to its row's share
     const float icap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     asm volatile("" : "+v"(slope));  // waited for here, not behind the loop's loads

@@ -183,3 +183,20 @@ def test_old_values_beside_slowly_rising_scores(gpu):
     o, bar = want(q[7], held("int8", c.k[at]), held("int8", c.v[at]), 1.0, 0.0, None)
     assert np.all(np.abs(got[7] - o) <= bar)
     assert not got[:7].any() and not got[8:].any()
+
+
+def test_large_queries_across_large_keys(gpu):
+    """Queries whose products with the keys' scales pass float32's range, and meet keys of zero: scores of 0."""
+    c = Case(gpu, "int8", 64, 1, [200, 33])
+    c.k *= np.float32(2.0 ** 30)
+    c.k[:, :, 9] = 0
+    put(c)
+    q = np.zeros((2, 4, 64), np.float32)
+    q[:, :, 9] = 2.0 ** 120
+    q[1, 2, 8] = 2.0 ** -30  # less than what the head's largest leaves of it: no score either
+    _, got = c.attend(4, q=q)
+    v = held("int8", c.v)
+    for r in range(2):
+        at = c.rows(r)
+        o, bar = want(np.zeros((4, 64), np.float32), 0 * v[at], v[at], 0.125, 0.0, None)
+        assert np.all(np.abs(got[r] - o) <= bar), r
